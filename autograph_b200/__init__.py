@@ -664,6 +664,83 @@ class _PyDevice:
                                        cols, inner, ctypes.c_float(beta), _ptr(out)))
         return out
 
+    # -- layer norm ------------------------------------------------------------------
+    def _norm_operands(self, x, weight, bias, shape):
+        """The normalised trailing shape (that of the weight, else `shape`, else the last dimension) and the number of
+        rows of x, after the checks that both directions share."""
+        if weight is not None:
+            shape = weight.shape
+        elif bias is not None:
+            shape = bias.shape
+        elif shape is None:
+            shape = x.shape[-1:]
+        shape = tuple(shape)
+        if not shape or len(shape) > x.dim() or tuple(x.shape[x.dim() - len(shape):]) != shape:
+            raise AgError(_capi.AG_ERR_SHAPE, f"layer_norm: the trailing shape of {tuple(x.shape)} is not {shape}")
+        for t, name in ((weight, "weight"), (bias, "bias")):
+            if t is None:
+                continue
+            if t.dtype != x.dtype:
+                raise AgError(_capi.AG_ERR_DTYPE, f"layer_norm: {name} is {t.dtype}, x is {x.dtype}")
+            if tuple(t.shape) != shape:
+                raise AgError(_capi.AG_ERR_SHAPE, f"layer_norm: {name} of shape {tuple(t.shape)}, expected {shape}")
+        cols = int(np.prod(shape, dtype=np.int64))
+        if cols == 0:
+            raise AgError(_capi.AG_ERR_SHAPE, "layer_norm: a row needs at least one value")
+        return shape, x.numel() // cols, cols
+
+    def _layer_norm(self, x, weight, bias, eps, shape, keep):
+        shape, rows, cols = self._norm_operands(x, weight, bias, shape)
+        code, f32 = _dtype_code(x.dtype), _torch().float32
+        x, weight, bias = self._sync_in(x, weight, bias)
+        y = self._out(tuple(x.shape), x.dtype)
+        lead = tuple(x.shape[:x.dim() - len(shape)])
+        mean, rstd = (self._out(lead, f32), self._out(lead, f32)) if keep else (None, None)
+        self._check(lib().ag_layer_norm_forward(
+            self._h, code, _ptr(x), _ptr(weight), _ptr(bias), rows, cols, ctypes.c_float(eps), _ptr(y), _ptr(mean),
+            _ptr(rstd)))
+        return y, mean, rstd
+
+    def layer_norm(self, x, weight=None, bias=None, eps=1e-5, shape=None):
+        """(x - mean) / sqrt(var + eps) * weight + bias over the trailing dimensions of x that
+        weight has (without one: `shape`, or the last dimension)."""
+        return self._layer_norm(x, weight, bias, eps, shape, False)[0]
+
+    def layer_norm_keep(self, x, weight=None, bias=None, eps=1e-5, shape=None):
+        """The same for a pass that records gradients: returns (y, mean, rstd), the last two f32
+        with the leading dimensions of x."""
+        return self._layer_norm(x, weight, bias, eps, shape, True)
+
+    def layer_norm_backward(self, x, dy, mean, rstd, weight=None, has_bias=False, shape=None, want_dx=True,
+                            beta=0.0, dweight=None, dbias=None):
+        """Gradients from the values layer_norm_keep kept: (dx or None, dweight or None, dbias or
+        None).  dweight and dbias given by the caller are written as beta * dweight + gradient."""
+        torch = _torch()
+        shape, rows, cols = self._norm_operands(x, weight, None, shape)
+        if tuple(dy.shape) != tuple(x.shape):
+            raise AgError(_capi.AG_ERR_SHAPE, f"layer_norm: dy of shape {tuple(dy.shape)}, x {tuple(x.shape)}")
+        for t, name, dt, n in ((dy, "dy", x.dtype, rows * cols), (mean, "mean", torch.float32, rows),
+                               (rstd, "rstd", torch.float32, rows), (dweight, "dweight", x.dtype, cols),
+                               (dbias, "dbias", x.dtype, cols)):
+            if t is None:
+                continue
+            if t.dtype != dt:
+                raise AgError(_capi.AG_ERR_DTYPE, f"layer_norm: {name} is {t.dtype}, expected {dt}")
+            if t.numel() != n:
+                raise AgError(_capi.AG_ERR_SHAPE, f"layer_norm: {name} has {t.numel()} values, expected {n}")
+        if beta != 0.0 and ((weight is not None and dweight is None) or (has_bias and dbias is None)):
+            raise AgError(_capi.AG_ERR_INVALID, "layer_norm: beta without the gradients that it scales")
+        x, dy, mean, rstd, weight = self._sync_in(x, dy, mean, rstd, weight, inout=(dweight, dbias))
+        dx = self._out(tuple(x.shape), x.dtype) if want_dx else None
+        if weight is not None and dweight is None:
+            dweight = self._out(shape, x.dtype)
+        if has_bias and dbias is None:
+            dbias = self._out(shape, x.dtype)
+        self._check(lib().ag_layer_norm_backward(
+            self._h, _dtype_code(x.dtype), _ptr(x), _ptr(weight), _ptr(mean), _ptr(rstd), _ptr(dy), rows, cols,
+            _ptr(dx), ctypes.c_float(beta), _ptr(dweight), _ptr(dbias)))
+        return dx, dweight, dbias
+
     # -- criterion -------------------------------------------------------------------
     def cross_entropy_loss(self, x, t) -> float:
         bs, classes = x.shape
@@ -720,6 +797,60 @@ class _PyDevice:
                                                  _ptr(v), w.numel(), ctypes.c_float(lr),
                                                  ctypes.c_float(momentum)))
         return w, v
+
+    @staticmethod
+    def _matrix_dtype(groups):
+        """All matrices of a call in one type, each of two dimensions or more."""
+        for name, tensors, dt in groups:
+            for t in tensors:
+                if t.dtype != dt:
+                    raise AgError(_capi.AG_ERR_DTYPE, f"newton_schulz: {name} is {t.dtype}, expected {dt}")
+                if t.dim() < 2:
+                    raise AgError(_capi.AG_ERR_SHAPE, f"newton_schulz: {name} of shape {tuple(t.shape)} is no matrix")
+                if t.numel() == 0:
+                    raise AgError(_capi.AG_ERR_SHAPE, "newton_schulz: a matrix needs at least one value")
+
+    def newton_schulz(self, gs, steps=5):
+        """Each gradient matrix of the list with its singular values taken to about one (`steps` Newton-Schulz
+        steps).  A tensor of more than two dimensions counts as [shape[0], rest], as a Conv2 filter bank does."""
+        gs = list(gs)
+        if not gs:
+            return []
+        self._matrix_dtype((("g", gs, gs[0].dtype),))
+        code = _dtype_code(gs[0].dtype)
+        gs = self._sync_in(*gs)
+        outs = [self._out(tuple(g.shape), g.dtype) for g in gs]
+        arr = (_capi.PolarMatrix * len(gs))()
+        for a, g, o in zip(arr, gs, outs):
+            a.g, a.o, a.rows, a.cols = g.data_ptr(), o.data_ptr(), g.shape[0], g.numel() // g.shape[0]
+        self._check(lib().ag_newton_schulz(self._h, code, len(gs), arr, steps))
+        return outs
+
+    def muon_update(self, ws, gs, vs, lr, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, scales=None):
+        """Muon's update of the parameters ws (lists of matrices, or of filter banks) in place: v = momentum * v + g,
+        w = (1 - lr * weight_decay) * w - lr * scale * newton_schulz(g + momentum * v).  vs are f32 whatever the
+        parameters' type; scales (default 1) one factor per matrix, e.g. sqrt(max(1, outputs / inputs))."""
+        torch = _torch()
+        ws, gs, vs = list(ws), list(gs), list(vs)
+        scales = [1.0] * len(ws) if scales is None else list(scales)
+        if not len(ws) == len(gs) == len(vs) == len(scales):
+            raise AgError(_capi.AG_ERR_SHAPE, "muon_update: lists of different lengths")
+        if not ws:
+            return ws, vs
+        self._matrix_dtype((("w", ws, ws[0].dtype), ("g", gs, ws[0].dtype), ("v", vs, torch.float32)))
+        for w, g, v in zip(ws, gs, vs):
+            if g.shape != w.shape or v.shape != w.shape:
+                raise AgError(_capi.AG_ERR_SHAPE, f"muon_update: w of shape {tuple(w.shape)}, g {tuple(g.shape)}, "
+                                                  f"v {tuple(v.shape)}")
+        code = _dtype_code(ws[0].dtype)
+        gs = self._sync_in(*gs, inout=(*ws, *vs))
+        arr = (_capi.MuonMatrix * len(ws))()
+        for a, w, g, v, scale in zip(arr, ws, gs, vs, scales):
+            a.w, a.g, a.v, a.scale = w.data_ptr(), g.data_ptr(), v.data_ptr(), scale
+            a.rows, a.cols = w.shape[0], w.numel() // w.shape[0]
+        self._check(lib().ag_muon_update(self._h, code, len(ws), arr, ctypes.c_float(lr), ctypes.c_float(momentum),
+                                         int(nesterov), ctypes.c_float(weight_decay), steps))
+        return ws, vs
 
 
 # Layer specs shared with the oracle's composition (kind, a, b, c, d, bias).

@@ -42,6 +42,15 @@ class LayerSpec(ctypes.Structure):
                 ("bias", c_int32)]
 
 
+class PolarMatrix(ctypes.Structure):
+    _fields_ = [("g", c_void_p), ("o", c_void_p), ("rows", c_int64), ("cols", c_int64)]
+
+
+class MuonMatrix(ctypes.Structure):
+    _fields_ = [("w", c_void_p), ("g", c_void_p), ("v", c_void_p), ("rows", c_int64), ("cols", c_int64),
+                ("scale", c_float)]
+
+
 def lib_path() -> Path:
     import os
     # AG_LIB: a side build of the same library (e.g. one with phase timestamps compiled in)
@@ -140,6 +149,11 @@ _SIGNATURES = {
     "ag_accuracy": (c_int, [_P, c_int, c_int, _P, _P, c_int64, c_int64, POINTER(c_uint64)]),
     "ag_sgd_update": (c_int, [_P, c_int, _P, _P, c_int64, c_float]),
     "ag_sgd_update_momentum": (c_int, [_P, c_int, _P, _P, _P, c_int64, c_float, c_float]),
+    "ag_layer_norm_forward": (c_int, [_P, c_int, _P, _P, _P, c_int64, c_int64, c_float, _P, _P, _P]),
+    "ag_layer_norm_backward": (c_int, [_P, c_int, _P, _P, _P, _P, _P, c_int64, c_int64, _P, c_float, _P, _P]),
+    "ag_newton_schulz": (c_int, [_P, c_int, c_int32, POINTER(PolarMatrix), c_int32]),
+    "ag_muon_update": (c_int, [_P, c_int, c_int32, POINTER(MuonMatrix), c_float, c_float, c_int, c_float,
+                               c_int32]),
     "ag_model_create": (c_int, [_P, c_int, POINTER(LayerSpec), c_int32, c_uint64, POINTER(_P)]),
     "ag_model_create_lenet5": (c_int, [_P, c_int, c_uint64, POINTER(_P)]),
     "ag_model_destroy": (c_int, [_P]),

@@ -381,6 +381,30 @@ AG_API int ag_bias_add(ag_device *dev, ag_dtype dtype, void *y, const void *bias
 AG_API int ag_bias_grad(ag_device *dev, ag_dtype dtype, const void *x, int64_t rows, int64_t cols,
                         int64_t inner, float beta, void *y);
 
+/* -------------------------------------------------------------- layer norm
+ * The reference has no normalisation layer; these two follow its operators' conventions.  x is
+ * viewed as [rows, cols], contiguous; weight and bias [cols] or NULL (ones and zeros).  Sums,
+ * statistics and products are f32, each result is rounded once.  A value that is not finite
+ * reaches its own row of y or dx and its columns of dweight and dbias, and nothing else. */
+
+/* Per row: mean = sum(x) / cols, rstd = 1 / sqrt(sum((x - mean)^2) / cols + eps),
+ * y = (x - mean) * rstd * weight + bias.  mean and rstd [rows] (f32) are what the backward pass
+ * reads; either may be NULL.  eps > 0.  y may be x, and must not overlap it otherwise. */
+AG_API int ag_layer_norm_forward(ag_device *dev, ag_dtype dtype, const void *x, const void *weight,
+                                 const void *bias, int64_t rows, int64_t cols, float eps, void *y,
+                                 float *mean, float *rstd);
+
+/* With hat = (x - mean) * rstd and d = dy * weight:
+ * dx = rstd * (d - sum(d) / cols - hat * sum(d * hat) / cols),
+ * dweight = beta * dweight + sum over rows of dy * hat, dbias = beta * dbias + sum over rows of
+ * dy (beta = 1 accumulates, beta = 0 does not read what was there; as in
+ * ag_conv2_backward_weight).  dx, dweight and dbias may each be NULL; dx must not overlap x or dy.
+ * The sums over rows are added in the same order on every call of the same sizes. */
+AG_API int ag_layer_norm_backward(ag_device *dev, ag_dtype dtype, const void *x, const void *weight,
+                                  const float *mean, const float *rstd, const void *dy,
+                                  int64_t rows, int64_t cols, void *dx, float beta, void *dweight,
+                                  void *dbias);
+
 /* -------------------------------------------------------------- criterion */
 
 /* ≙ cross_entropy_loss_device + kernels::cross_entropy_loss_<X>_<T> + sum
@@ -427,6 +451,41 @@ AG_API int ag_sgd_update(ag_device *dev, ag_dtype dtype, void *w, const void *g,
  * v = m*v + g; w -= lr*v in f32, stored back in T. */
 AG_API int ag_sgd_update_momentum(ag_device *dev, ag_dtype dtype, void *w, const void *g, void *v,
                                   int64_t n, float lr, float momentum);
+
+/* One matrix of ag_newton_schulz: g and o [rows, cols], contiguous.  o may be g. */
+typedef struct ag_polar_matrix {
+    const void *g;
+    void *o;
+    int64_t rows, cols;
+} ag_polar_matrix;
+
+/* Orthogonalises n gradient matrices: o = the result of `steps` Newton-Schulz steps
+ * x <- 3.4445 x - 4.7750 (x x^T) x + 2.0315 (x x^T)^2 x from x = g / norm(g) (Frobenius norm; the
+ * shorter side multiplies), which takes the singular values of g / norm(g) to about one.  A
+ * matrix of zeros gives zeros; one that holds a value that is not finite gives NaN.  Products
+ * and norms are held to f32 precision for AG_F32 and well inside the result's rounding for
+ * AG_BF16.  steps in 1..20, n in 0..4096, the shorter side in 1..16384, the longer up to 2^20 and
+ * fewer than 2^31 values per matrix; no o overlaps another matrix. */
+AG_API int ag_newton_schulz(ag_device *dev, ag_dtype dtype, int32_t n,
+                            const ag_polar_matrix *matrices, int32_t steps);
+
+/* One parameter of ag_muon_update: w and g [rows, cols] of the call's dtype, v [rows, cols] f32,
+ * all contiguous. */
+typedef struct ag_muon_matrix {
+    void *w;
+    const void *g;
+    float *v;
+    int64_t rows, cols;
+    float scale;
+} ag_muon_matrix;
+
+/* Muon's update of n parameters, beside ag_sgd_update_momentum for those that are matrices:
+ * v = momentum * v + g; u = nesterov ? g + momentum * v : v; o = the orthogonalised u
+ * (ag_newton_schulz, u not rounded); w = (1 - lr * weight_decay) * w - lr * scale * o, rounded
+ * once.  Limits as for ag_newton_schulz; every w and v is a buffer of its own.  v stays f32 for
+ * AG_BF16: a momentum near one adds gradients that are less than half a bf16 step of it. */
+AG_API int ag_muon_update(ag_device *dev, ag_dtype dtype, int32_t n, const ag_muon_matrix *matrices,
+                          float lr, float momentum, int nesterov, float weight_decay, int32_t steps);
 
 /* --------------------------------------------------- neural-network layer
  * Host-side mirror of the reference's Layer / Forward objects for the

@@ -57,6 +57,26 @@ pub struct ag_layer_spec {
     pub bias: i32,
 }
 
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct ag_polar_matrix {
+    pub g: *const c_void,
+    pub o: *mut c_void,
+    pub rows: i64,
+    pub cols: i64,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct ag_muon_matrix {
+    pub w: *mut c_void,
+    pub g: *const c_void,
+    pub v: *mut f32,
+    pub rows: i64,
+    pub cols: i64,
+    pub scale: f32,
+}
+
 #[link(name = "autograph_b200")]
 extern "C" {
     pub fn ag_last_error() -> *const c_char;
@@ -105,6 +125,8 @@ extern "C" {
     pub fn ag_scaled_add(dev: *mut ag_device, dtype: c_int, alpha: f32, x: *const c_void, y: *mut c_void, n: i64) -> c_int;
     pub fn ag_bias_add(dev: *mut ag_device, dtype: c_int, y: *mut c_void, bias: *const c_void, rows: i64, cols: i64, inner: i64) -> c_int;
     pub fn ag_bias_grad(dev: *mut ag_device, dtype: c_int, x: *const c_void, rows: i64, cols: i64, inner: i64, beta: f32, y: *mut c_void) -> c_int;
+    pub fn ag_layer_norm_forward(dev: *mut ag_device, dtype: c_int, x: *const c_void, weight: *const c_void, bias: *const c_void, rows: i64, cols: i64, eps: f32, y: *mut c_void, mean: *mut f32, rstd: *mut f32) -> c_int;
+    pub fn ag_layer_norm_backward(dev: *mut ag_device, dtype: c_int, x: *const c_void, weight: *const c_void, mean: *const f32, rstd: *const f32, dy: *const c_void, rows: i64, cols: i64, dx: *mut c_void, beta: f32, dweight: *mut c_void, dbias: *mut c_void) -> c_int;
     pub fn ag_cross_entropy_loss(dev: *mut ag_device, dtype: c_int, label_dtype: c_int, x: *const c_void, t: *const c_void, bs: i64, classes: i64, loss_host: *mut f32) -> c_int;
     pub fn ag_cross_entropy_loss_device(dev: *mut ag_device, dtype: c_int, label_dtype: c_int, x: *const c_void, t: *const c_void, bs: i64, classes: i64, loss_dev: *mut f32) -> c_int;
     pub fn ag_cross_entropy_loss_device_grad(dev: *mut ag_device, dtype: c_int, label_dtype: c_int, x: *const c_void, t: *const c_void, bs: i64, classes: i64, loss_dev: *mut f32, dy: f32, dx: *mut c_void) -> c_int;
@@ -112,6 +134,8 @@ extern "C" {
     pub fn ag_accuracy(dev: *mut ag_device, dtype: c_int, label_dtype: c_int, x: *const c_void, t: *const c_void, bs: i64, classes: i64, correct_host: *mut u64) -> c_int;
     pub fn ag_sgd_update(dev: *mut ag_device, dtype: c_int, w: *mut c_void, g: *const c_void, n: i64, lr: f32) -> c_int;
     pub fn ag_sgd_update_momentum(dev: *mut ag_device, dtype: c_int, w: *mut c_void, g: *const c_void, v: *mut c_void, n: i64, lr: f32, momentum: f32) -> c_int;
+    pub fn ag_newton_schulz(dev: *mut ag_device, dtype: c_int, n: i32, matrices: *const ag_polar_matrix, steps: i32) -> c_int;
+    pub fn ag_muon_update(dev: *mut ag_device, dtype: c_int, n: i32, matrices: *const ag_muon_matrix, lr: f32, momentum: f32, nesterov: c_int, weight_decay: f32, steps: i32) -> c_int;
     pub fn ag_model_create(dev: *mut ag_device, dtype: c_int, layers: *const ag_layer_spec, n_layers: i32, seed: u64, out: *mut *mut ag_model) -> c_int;
     pub fn ag_model_create_lenet5(dev: *mut ag_device, dtype: c_int, seed: u64, out: *mut *mut ag_model) -> c_int;
     pub fn ag_model_destroy(model: *mut ag_model) -> c_int;

@@ -17,7 +17,7 @@ TYPES = {
     "uint32_t": "u32", "size_t": "usize", "float": "f32", "double": "f64", "void": "c_void",
     "char": "c_char", "ag_dtype": "c_int", "ag_device": "ag_device", "ag_model": "ag_model",
     "ag_comm": "ag_comm", "ag_conv2_options": "ag_conv2_options", "ag_conv_stage": "ag_conv_stage",
-    "ag_layer_spec": "ag_layer_spec",
+    "ag_layer_spec": "ag_layer_spec", "ag_polar_matrix": "ag_polar_matrix", "ag_muon_matrix": "ag_muon_matrix",
 }
 
 
@@ -115,6 +115,26 @@ def main():
         "    pub c: i32,",
         "    pub d: i32,",
         "    pub bias: i32,",
+        "}",
+        "",
+        "#[repr(C)]",
+        "#[derive(Clone, Copy)]",
+        "pub struct ag_polar_matrix {",
+        "    pub g: *const c_void,",
+        "    pub o: *mut c_void,",
+        "    pub rows: i64,",
+        "    pub cols: i64,",
+        "}",
+        "",
+        "#[repr(C)]",
+        "#[derive(Clone, Copy)]",
+        "pub struct ag_muon_matrix {",
+        "    pub w: *mut c_void,",
+        "    pub g: *const c_void,",
+        "    pub v: *mut f32,",
+        "    pub rows: i64,",
+        "    pub cols: i64,",
+        "    pub scale: f32,",
         "}",
         "",
         '#[link(name = "autograph_b200")]',
