@@ -3,152 +3,116 @@
 // With x = u / norm(u), as n x m with n <= m (the transpose of a taller u), a step is
 //   a = x x^T,  b = B a + C a a,  x <- A x + b x,   (A, B, C) = (3.4445, -4.7750, 2.0315),
 // which maps every singular value s to A s + B s^3 + C s^5 and keeps the singular vectors.
-#include "common.cuh"
-
 #include <algorithm>
 #include <vector>
+
+#include "muon_product.cuh"
 
 namespace ag {
 namespace muon {
 
-constexpr float kA = 3.4445f, kB = -4.7750f, kC = 2.0315f;
 constexpr int64_t kMostShort = 16384, kMostLong = 1 << 20;
 constexpr int kMostMatrices = 4096, kMostSteps = 20;
-constexpr int kNormParts = 64;   // partial sums of squares of a matrix
+constexpr int kMostParts = 2048;              // partial sums of squares of a matrix
+constexpr int64_t kInside = 1 << 20;          // values of a launch up to which its one kernel does everything
 
-// One matrix of a call.
-struct Matrix {
-    const void *g;
-    void *o;        // result, or the weight that it updates
-    float *v;       // momentum, or null
-    int64_t rows, cols;
-    float scale;
-};
-
-// The update's scalars.
-struct Rule {
-    float lr, momentum, decay;
-    int nesterov;
-};
-
-// u from the gradient and, for an update, the momentum after it.
-template <class T>
-__device__ __forceinline__ float direction(const Matrix &m, const Rule &r, int64_t i) {
-    const float g = to_f32(reinterpret_cast<const T *>(m.g)[i]);
-    if (m.v == nullptr) return g;
-    const float v = m.v[i];
-    return r.nesterov ? fmaf(r.momentum, v, g) : v;
+// The CTA's matrix, of which it takes the `count(m)`-th piece.
+template <class F>
+__device__ __forceinline__ int find_matrix(const Group &g, int &piece, F count) {
+    int i = 0;
+    for (piece = blockIdx.x; i + 1 < g.n && piece >= count(g.m[i]); ++i) piece -= count(g.m[i]);
+    return i;
 }
 
-// v = momentum * v + g, and partial sums of u^2 in f64 (u^2 itself can exceed f32's range).
 template <class T>
-__global__ void __launch_bounds__(256) momentum_kernel(const Matrix m, const Rule r, double *parts) {
+__global__ void __launch_bounds__(256) momentum_kernel(const __grid_constant__ Group g, double *parts) {
     __shared__ double scratch[8];
-    let_dependents_launch();
-    dependency_wait();
-    const int64_t n = m.rows * m.cols;
-    double s = 0;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        if (m.v != nullptr) m.v[i] = __fadd_rn(__fmul_rn(r.momentum, m.v[i]), to_f32(reinterpret_cast<const T *>(m.g)[i]));
-        const double u = direction<T>(m, r, i);
-        s += u * u;
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (threadIdx.x % 32 == 0) scratch[threadIdx.x / 32] = s;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int i = 1; i < 8; ++i) s += scratch[i];
-        parts[blockIdx.x] = s;
-    }
+    int part;
+    const int i = find_matrix(g, part, [](const Matrix &m) { return m.parts; });
+    momentum_part<T>(g.m[i], g.rule, part, parts, scratch);
 }
 
-// x = u / norm(u), transposed where u is taller than wide.  A norm of zero gives zeros, one that is not finite NaN.
 template <class T>
-__global__ void __launch_bounds__(256) scale_kernel(const Matrix m, const Rule r, const double *parts, float *x) {
-    let_dependents_launch();
-    dependency_wait();
-    double s = 0;
-    for (int i = 0; i < kNormParts; ++i) s += parts[i];
-    const double inv = s == 0 ? 0. : isfinite(s) ? 1. / sqrt(s) : (double)NAN;
-    const bool flip = m.rows > m.cols;
-    const int64_t n = m.rows * m.cols, wide = flip ? m.rows : m.cols;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        const int64_t row = i / wide, col = i - row * wide;
-        x[i] = (float)(direction<T>(m, r, flip ? col * m.cols + row : i) * inv);
-    }
+__global__ void __launch_bounds__(256) split_kernel(const __grid_constant__ Group g, const double *parts, __half *planes) {
+    __shared__ double scratch[8];
+    __shared__ float tile[64][65];
+    int block;
+    const int i = find_matrix(g, block, [](const Matrix &m) { return m.x.plane / 64; });
+    const double inv = inverse_norm(g.m[i], parts, scratch);
+    split_tile<T>(g.m[i], g.rule, block, inv, planes, tile);
 }
 
-// c = p * (a . b) + q * e, row-major f32: a [M, K], b [K, N], or [N, K] when bt; 32 x 32 outputs a CTA.
-__global__ void __launch_bounds__(256)
-    product_kernel(const float *a, const float *b, bool bt, int M, int N, int K, float p, float q, const float *e, float *c) {
-    __shared__ float sa[32][33], sb[32][33];
-    let_dependents_launch();
-    dependency_wait();
-    const int m0 = blockIdx.y * 32, n0 = blockIdx.x * 32, tx = threadIdx.x % 32, ty = threadIdx.x / 32;
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int k0 = 0; k0 < K; k0 += 32) {
-        for (int i = ty; i < 32; i += 8) {
-            sa[i][tx] = m0 + i < M && k0 + tx < K ? a[(int64_t)(m0 + i) * K + k0 + tx] : 0.f;
-            if (bt)
-                sb[tx][i] = n0 + i < N && k0 + tx < K ? b[(int64_t)(n0 + i) * K + k0 + tx] : 0.f;
-            else
-                sb[i][tx] = n0 + tx < N && k0 + i < K ? b[(int64_t)(k0 + i) * N + n0 + tx] : 0.f;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < 32; ++k)
-            for (int j = 0; j < 4; ++j) acc[j] = fmaf(sa[ty + 8 * j][k], sb[k][tx], acc[j]);
-        __syncthreads();
+// Rows of the workspace, handed out.
+struct Space {
+    int64_t rows = 0;
+    Stored take(int64_t r, int64_t c) {
+        Stored s;
+        s.rp = (int)(ceil_div(r, 128) * 128);
+        s.plane = (int)(ceil_div(c, 64) * s.rp);
+        s.row = (int)rows;
+        rows += 2 * (int64_t)s.plane;
+        return s;
     }
-    for (int j = 0; j < 4; ++j) {
-        const int64_t i = (int64_t)(m0 + ty + 8 * j) * N + n0 + tx;
-        if (m0 + ty + 8 * j < M && n0 + tx < N) c[i] = q != 0.f ? fmaf(p, acc[j], q * e[i]) : p * acc[j];
-    }
-}
-
-// o = x, or w = (1 - lr * decay) * w - lr * scale * x.
-template <class T>
-__global__ void __launch_bounds__(256) store_kernel(const Matrix m, const Rule r, const float *x) {
-    let_dependents_launch();
-    dependency_wait();
-    const bool flip = m.rows > m.cols;
-    const int64_t n = m.rows * m.cols, wide = flip ? m.rows : m.cols;
-    T *o = reinterpret_cast<T *>(m.o);
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        const int64_t row = i / m.cols, col = i - row * m.cols;
-        const float v = flip ? x[col * wide + row] : x[i];
-        o[i] = from_f32<T>(m.v == nullptr ? v : fmaf(-r.lr * m.scale, v, (1.f - r.lr * r.decay) * to_f32(o[i])));
-    }
-}
+};
 
 template <class T>
 int run(ag_device *dev, const std::vector<Matrix> &matrices, const Rule &rule, int steps) {
-    int64_t most = 0;
-    for (const Matrix &m : matrices) {
-        const int64_t n = std::min(m.rows, m.cols);
-        most = std::max(most, 2 * m.rows * m.cols + 2 * n * n);
-    }
-    void *ws;
-    AG_TRY(workspace(dev, kNormParts * sizeof(double) + (size_t)most * sizeof(float), &ws));
-    double *parts = (double *)ws;
-    for (const Matrix &mat : matrices) {
-        const int64_t n = std::min(mat.rows, mat.cols), m = std::max(mat.rows, mat.cols);
-        float *x = (float *)(parts + kNormParts), *y = x + n * m, *a = y + n * m, *b = a + n * n;
-        const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(n * m, 256), 8 * dev->sm_count);
-        AG_TRY(launch_dependent(dev, momentum_kernel<T>, dim3(kNormParts), 256, 0, mat, rule, parts));
-        AG_TRY(launch_dependent(dev, scale_kernel<T>, dim3(grid), 256, 0, mat, rule, (const double *)parts, x));
-        const dim3 square((unsigned)ceil_div(n, 32), (unsigned)ceil_div(n, 32)), wide((unsigned)ceil_div(m, 32), square.y);
-        for (int s = 0; s < steps; ++s) {
-            AG_TRY(launch_dependent(dev, product_kernel, square, 256, 0, (const float *)x, (const float *)x, true, (int)n, (int)n,
-                                    (int)m, 1.f, 0.f, (const float *)nullptr, a));
-            AG_TRY(launch_dependent(dev, product_kernel, square, 256, 0, (const float *)a, (const float *)a, false, (int)n, (int)n,
-                                    (int)n, kC, kB, (const float *)a, b));
-            AG_TRY(launch_dependent(dev, product_kernel, wide, 256, 0, (const float *)b, (const float *)x, false, (int)n, (int)m,
-                                    (int)n, 1.f, kA, (const float *)x, y));
-            std::swap(x, y);
+    for (size_t first = 0; first < matrices.size(); first += kGroup) {
+        Group g = {};
+        g.n = (int)std::min<size_t>(kGroup, matrices.size() - first);
+        g.steps = steps;
+        g.rule = rule;
+        Space space;
+        int parts = 0, blocks = 0;
+        int64_t values = 0;
+        for (int i = 0; i < g.n; ++i) {
+            Matrix &m = g.m[i];
+            m = matrices[first + i];
+            const int64_t n = std::min(m.rows, m.cols), wide = std::max(m.rows, m.cols);
+            m.x = space.take(n, wide);
+            m.y = space.take(n, wide);
+            m.a = space.take(n, n);
+            m.b = space.take(n, n);
+            m.part0 = parts;
+            m.parts = (int)std::min<int64_t>(ceil_div(n * wide, 8192), kMostParts);
+            parts += m.parts;
+            blocks += m.x.plane / 64;
+            values += n * wide;
         }
-        AG_TRY(launch_dependent(dev, store_kernel<T>, dim3(grid), 256, 0, mat, rule, (const float *)x));
+        AG_REQUIRE(space.rows < (1ll << 31), AG_ERR_LIMIT, "newton_schulz: the matrices' workspace is too large");
+        g.inside = values <= kInside;
+        const size_t heads = (size_t)kGroup * kMostParts * sizeof(double), sums = (size_t)dev->sm_count * 128 * 128 * sizeof(float);
+        void *ws;
+        AG_TRY(engine_scratch(dev, heads + sums + (size_t)space.rows * 128, &ws));
+        double *norms = (double *)ws;
+        float *slices = (float *)((char *)ws + heads);
+        __half *planes = (__half *)((char *)ws + heads + sums);
+        CUtensorMap map;
+        const uint64_t dims[2] = {64, (uint64_t)space.rows}, strides[1] = {64};
+        const uint32_t box[2] = {64, 64};
+        AG_TRY(make_tmap_bf16(&map, planes, 2, dims, strides, box));   // f16 has the same size
+        if (!g.inside) {
+            momentum_kernel<T><<<parts, 256, 0, dev->stream>>>(g, norms);
+            AG_CHECK_LAUNCH();
+            split_kernel<T><<<blocks, 256, 0, dev->stream>>>(g, norms, planes);
+            AG_CHECK_LAUNCH();
+        }
+        auto kernel = muon_kernel<T>;
+        static SmemAllowed allowed;
+        AG_TRY(allow_smem<kSmem>(dev, kernel, allowed));
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)dev->sm_count);
+        cfg.blockDim = kThreads;
+        cfg.dynamicSmemBytes = kSmem;
+        cfg.stream = dev->stream;
+        // the grid's barrier needs all CTAs at once
+        cudaLaunchAttribute attr;
+        attr.id = cudaLaunchAttributeCooperative;
+        attr.val.cooperative = 1;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        AG_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, map, planes, norms, slices, dev->tile_counters, dev->status_dev, g));
+        AG_CHECK_LAUNCH();
     }
     return AG_OK;
 }
@@ -211,7 +175,7 @@ int ag_newton_schulz(ag_device *dev, ag_dtype dtype, int32_t n, const ag_polar_m
             const uintptr_t bytes = (uintptr_t)(m.rows * m.cols) * dtype_size(dtype);
             ranges.push_back({(uintptr_t)m.g, (uintptr_t)m.g + bytes, false, i, true});
             ranges.push_back({(uintptr_t)m.o, (uintptr_t)m.o + bytes, true, i, true});
-            list.push_back({m.g, m.o, nullptr, m.rows, m.cols, 1.f});
+            list.push_back({m.g, m.o, nullptr, m.rows, m.cols, 1.f, 0, 0, {}, {}, {}, {}});
         }
         AG_TRY(muon::check_overlap(ranges));
         const muon::Rule rule = {0.f, 0.f, 0.f, 0};
@@ -237,7 +201,7 @@ int ag_muon_update(ag_device *dev, ag_dtype dtype, int32_t n, const ag_muon_matr
             ranges.push_back({(uintptr_t)m.g, (uintptr_t)m.g + bytes, false, i, false});
             ranges.push_back({(uintptr_t)m.w, (uintptr_t)m.w + bytes, true, i, false});
             ranges.push_back({(uintptr_t)m.v, (uintptr_t)m.v + count * 4, true, i, false});
-            list.push_back({m.g, m.w, m.v, m.rows, m.cols, m.scale});
+            list.push_back({m.g, m.w, m.v, m.rows, m.cols, m.scale, 0, 0, {}, {}, {}, {}});
         }
         AG_TRY(muon::check_overlap(ranges));
         const muon::Rule rule = {lr, momentum, weight_decay, nesterov ? 1 : 0};

@@ -1,0 +1,655 @@
+// The Newton-Schulz steps of a list of matrices as one kernel: a CTA per SM that goes through the steps' products phase by
+// phase, D = c0 * (P . Q) + c1 * E on tcgen05, with a barrier of the whole grid between two phases.
+//
+// Matrices live in one workspace as f16 planes.  A value x is held as hi + lo, hi = f16(x * 2^k) and lo = f16 of what
+// that leaves: 22 bits, of which a product takes hi.hi + hi.lo + lo.hi (what is dropped is 2^-24 of a product at most, as
+// f32's own rounding), or hi.hi alone where eleven bits are enough.  The scales 2^k are fixed, because the values are
+// bounded: the singular values of every x of the iteration stay below 1.21.
+//
+// A matrix of R x C is stored in panels of 64 columns, [C / 64][Rp][64] with Rp = R rounded up to 128 and zeros in the
+// padding, so that a panel's rows are 128 bytes: the whole workspace is one matrix of 128-byte rows behind one tensor map,
+// and a box of 64 rows is a tile of the operand, K-major where the product runs along the columns and MN-major where it
+// runs along the rows.
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include "tc_ptx.cuh"
+
+namespace ag {
+namespace muon {
+
+// A stored matrix: its first row in the workspace, rows of a panel, rows of a plane.
+struct Stored {
+    int row, rp, plane;
+};
+
+// One matrix of a call.
+struct Matrix {
+    const void *g;
+    void *o;        // result, or the weight that it updates
+    float *v;       // momentum, or null
+    int64_t rows, cols;
+    float scale;
+    int part0, parts;   // its partial sums of squares
+    Stored x, y, a, b;
+};
+
+// The update's scalars.
+struct Rule {
+    float lr, momentum, decay;
+    int nesterov;
+};
+
+constexpr int kGroup = 24;   // matrices of a launch: its parameters stay below 4 KB
+struct Group {
+    int n, steps;
+    int inside;              // the kernel makes the momenta, norms and planes too
+    Rule rule;
+    Matrix m[kGroup];
+};
+
+// One product.
+struct Job {
+    Stored p, q, e, d;
+    int q_mn;          // q's rows run along the product's depth
+    int M, N;          // of D
+    int steps;         // 64-k steps
+    int symmetric;     // D is: only tiles on and above the diagonal are computed
+    int has_e, final;
+    int planes;        // of each operand: 2 for hi.hi + hi.lo + lo.hi, 1 for hi.hi
+    float c0, c1;
+};
+
+constexpr float kA = 3.4445f, kB = -4.7750f, kC = 2.0315f;
+// Scales of the stored matrices.  |x| <= 1.21, |a| <= 1.46 and |b| <= 2.81 by their norms, f16 ends at 65504.
+constexpr float kScaleX = 32768.f, kScaleA = 32768.f, kScaleB = 16384.f;
+
+using namespace tc;
+
+// ---- epilogue ------------------------------------------------------------------------------------
+
+__device__ __forceinline__ int64_t at(const Stored &m, int row, int col) {
+    return ((int64_t)m.row + (int64_t)(col / 64) * m.rp + row) * 64 + col % 64;
+}
+
+// Eight neighbouring values of one row as two f16 planes.
+__device__ __forceinline__ void split8(const float (&v)[8], uint4 &hi, uint4 &lo) {
+    uint32_t h[4], l[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __half2 a = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+        const float2 f = __half22float2(a);
+        const __half2 b = __floats2half2_rn(v[2 * i] - f.x, v[2 * i + 1] - f.y);
+        h[i] = *reinterpret_cast<const uint32_t *>(&a);
+        l[i] = *reinterpret_cast<const uint32_t *>(&b);
+    }
+    hi = make_uint4(h[0], h[1], h[2], h[3]);
+    lo = make_uint4(l[0], l[1], l[2], l[3]);
+}
+__device__ __forceinline__ void join8(const uint4 &hi, const uint4 &lo, float (&v)[8]) {
+    const uint32_t h[4] = {hi.x, hi.y, hi.z, hi.w}, l[4] = {lo.x, lo.y, lo.z, lo.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&h[i]));
+        const float2 b = __half22float2(*reinterpret_cast<const __half2 *>(&l[i]));
+        v[2 * i] = a.x + b.x;
+        v[2 * i + 1] = a.y + b.y;
+    }
+}
+
+// o = x, or w = (1 - lr * decay) * w - lr * scale * x.
+template <class T>
+__device__ __forceinline__ void store_final(const Matrix &m, const Rule &r, int M, int N, int row, int col, const float (&v)[8]) {
+    T *o = reinterpret_cast<T *>(m.o);
+    if (row >= M) return;
+    const bool flip = m.rows > m.cols, update = m.v != nullptr;
+    const float keep = 1.f - r.lr * r.decay, step = -r.lr * m.scale;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (col + i < N) {
+            T *p = flip ? o + (int64_t)(col + i) * m.cols + row : o + (int64_t)row * m.cols + col + i;
+            *p = from_f32<T>(update ? fmaf(step, v[i], keep * to_f32(*p)) : v[i]);
+        }
+}
+
+// Columns col .. col + 7 (col a multiple of 8) of a row of D from their sums.  `mirror`: also the transposed place.
+// What another SM has stored in this launch is read past the SM's own cache.
+template <class T>
+__device__ __forceinline__ void finish8(const Job &j, const Matrix &m, const Rule &r, __half *planes, int row, int col,
+                                        float (&v)[8], bool mirror) {
+    if (row >= (j.M + 127) / 128 * 128 || col >= (j.N + 63) / 64 * 64) return;
+    if (j.has_e) {
+        const int64_t i = at(j.e, row, col);
+        float e[8];
+        join8(__ldcg(reinterpret_cast<const uint4 *>(planes + i)),
+              __ldcg(reinterpret_cast<const uint4 *>(planes + i + (int64_t)j.e.plane * 64)), e);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = fmaf(j.c0, v[k], j.c1 * e[k]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] *= j.c0;
+    }
+    if (j.final) {
+        store_final<T>(m, r, j.M, j.N, row, col, v);
+        return;
+    }
+    uint4 hi, lo;
+    split8(v, hi, lo);
+    const int64_t i = at(j.d, row, col), plane = (int64_t)j.d.plane * 64;
+    *reinterpret_cast<uint4 *>(planes + i) = hi;
+    *reinterpret_cast<uint4 *>(planes + i + plane) = lo;
+    if (mirror) {
+        const uint32_t h[4] = {hi.x, hi.y, hi.z, hi.w}, l[4] = {lo.x, lo.y, lo.z, lo.w};
+        unsigned short *m = reinterpret_cast<unsigned short *>(planes) + at(j.d, col, row);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            m[k * 64] = (unsigned short)(h[k / 2] >> (k % 2 * 16));
+            m[k * 64 + plane] = (unsigned short)(l[k / 2] >> (k % 2 * 16));
+        }
+    }
+}
+
+// ---- before the steps ------------------------------------------------------------------------------
+
+// u from the gradient and, for an update, the momentum after it.
+template <class T>
+__device__ __forceinline__ float direction(const Matrix &m, const Rule &r, int64_t i) {
+    const float g = to_f32(reinterpret_cast<const T *>(m.g)[i]);
+    if (m.v == nullptr) return g;
+    const float v = __ldcg(m.v + i);
+    return r.nesterov ? fmaf(r.momentum, v, g) : v;
+}
+
+// Sum over the CTA's threads, to all of them; the same order on every run.
+__device__ __forceinline__ double cta_sum(double s, double *scratch) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    __syncthreads();
+    if (threadIdx.x % 32 == 0) scratch[threadIdx.x / 32] = s;
+    __syncthreads();
+    s = 0;
+    for (int i = 0; i < (int)blockDim.x / 32; ++i) s += scratch[i];
+    return s;
+}
+
+// v = momentum * v + g over one part of a matrix, and the part's sum of u^2 in f64 (u^2 itself can exceed f32's range).
+template <class T>
+__device__ __forceinline__ void momentum_part(const Matrix &m, const Rule &r, int part, double *parts, double *scratch) {
+    const int64_t n = m.rows * m.cols, per = (n + m.parts - 1) / m.parts, first = part * per, last = min(n, first + per);
+    double s = 0;
+    for (int64_t i = first + threadIdx.x; i < last; i += blockDim.x) {
+        float u = to_f32(reinterpret_cast<const T *>(m.g)[i]);
+        if (m.v != nullptr) {
+            const float v = __fadd_rn(__fmul_rn(r.momentum, m.v[i]), u);
+            m.v[i] = v;
+            u = r.nesterov ? fmaf(r.momentum, v, u) : v;
+        }
+        s += (double)u * (double)u;
+    }
+    s = cta_sum(s, scratch);
+    if (threadIdx.x == 0) parts[m.part0 + part] = s;
+}
+
+// kScaleX / norm(u).  A norm of zero gives zeros, one that is not finite NaN.
+__device__ __forceinline__ double inverse_norm(const Matrix &m, const double *parts, double *scratch) {
+    double s = 0;
+    for (int i = threadIdx.x; i < m.parts; i += blockDim.x) s += __ldcg(parts + m.part0 + i);
+    s = cta_sum(s, scratch);
+    return s == 0 ? 0. : isfinite(s) ? (double)kScaleX / sqrt(s) : (double)NAN;
+}
+
+// 64 x 64 values of x = u / norm(u), transposed where u is taller than wide, as planes.
+template <class T>
+__device__ __forceinline__ void split_tile(const Matrix &m, const Rule &r, int block, double inv, __half *planes,
+                                           float (*tile)[65]) {
+    const bool flip = m.rows > m.cols;
+    const int N = (int)(flip ? m.cols : m.rows), M = (int)(flip ? m.rows : m.cols), tiles = m.x.rp / 64;
+    const int i0 = block % tiles * 64, j0 = block / tiles * 64;
+    for (int t = threadIdx.x; t < 64 * 64; t += blockDim.x) {
+        const int inner = t % 64, outer = t / 64, i = i0 + (flip ? inner : outer), j = j0 + (flip ? outer : inner);
+        float x = 0.f;
+        if (i < N && j < M) x = (float)(direction<T>(m, r, flip ? (int64_t)j * m.cols + i : (int64_t)i * m.cols + j) * inv);
+        tile[i - i0][j - j0] = x;
+    }
+    __syncthreads();
+    for (int t = threadIdx.x; t < 64 * 8; t += blockDim.x) {
+        const int i = t / 8, c = t % 8 * 8;
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = tile[i][c + k];
+        uint4 hi, lo;
+        split8(v, hi, lo);
+        const int64_t to = at(m.x, i0 + i, j0 + c);
+        *reinterpret_cast<uint4 *>(planes + to) = hi;
+        *reinterpret_cast<uint4 *>(planes + to + (int64_t)m.x.plane * 64) = lo;
+    }
+    __syncthreads();
+}
+
+// ---- the steps --------------------------------------------------------------------------------------
+
+constexpr int kEpiWarps = 8, kThreads = 64 + kEpiWarps * 32;
+constexpr int kBox = 64 * 64 * 2;          // bytes of a box of the tensor map
+constexpr int kHalf = 4 * kBox;            // 128 rows of P and of Q, 64 k, one plane
+constexpr int kStage = 2 * kHalf, kStages = 3;   // both planes of 64 k, or the upper one of 128
+constexpr int kSmem = kStages * kStage + 1024 + 512;
+
+// Products of planes of a step.  bf16 results: the products of the last step and of those before the last three are of the
+// planes' upper halves alone.  What an early step rounds off is later drawn to one with the singular values; what the last
+// one does is 2^-12 of its operands and not multiplied any more.  Short sides average too little for that, and their
+// products cost nothing.
+__device__ __forceinline__ int planes_of(bool bf16, int n, int step, int steps) {
+    const int left = steps - 1 - step;
+    return bf16 && n >= 128 && (left == 0 || left > 2) ? 1 : 2;
+}
+
+// Product `phase` (three a step) of a matrix.
+template <class T>
+__device__ __forceinline__ Job make_job(const Matrix &m, int phase, int steps) {
+    const int s = phase / 3, n = (int)min(m.rows, m.cols), long_side = (int)max(m.rows, m.cols);
+    const Stored x = s % 2 == 0 ? m.x : m.y, y = s % 2 == 0 ? m.y : m.x;
+    Job j;
+    j.planes = planes_of(sizeof(T) == 2, n, s, steps);
+    j.final = 0;
+    j.M = n;
+    if (phase % 3 == 0) {          // a = x x^T
+        j.p = j.q = j.e = x;
+        j.d = m.a;
+        j.q_mn = 0;
+        j.N = n;
+        j.steps = (long_side + 63) / 64;
+        j.symmetric = 1;
+        j.has_e = 0;
+        j.c0 = kScaleA / (kScaleX * kScaleX);
+        j.c1 = 0.f;
+    } else if (phase % 3 == 1) {   // b = B a + C a a
+        j.p = j.q = j.e = m.a;
+        j.d = m.b;
+        j.q_mn = 0;
+        j.N = n;
+        j.steps = (n + 63) / 64;
+        j.symmetric = 1;
+        j.has_e = 1;
+        j.c0 = kC * kScaleB / (kScaleA * kScaleA);
+        j.c1 = kB * kScaleB / kScaleA;
+    } else {                       // x = A x + b x
+        j.p = m.b;
+        j.q = j.e = x;
+        j.d = y;
+        j.q_mn = 1;
+        j.N = long_side;
+        j.steps = (n + 63) / 64;
+        j.symmetric = 0;
+        j.has_e = 1;
+        j.final = s + 1 == steps;
+        j.c0 = 1.f / (kScaleB * (j.final ? kScaleX : 1.f));
+        j.c1 = j.final ? kA / kScaleX : kA;
+    }
+    return j;
+}
+
+// The work items of a phase: tiles of 128 x 128, of all matrices in a row, each cut in `splits` slices of its depth.
+struct Plan {
+    int items, splits;
+    int first[kGroup + 1];   // of each matrix's tiles
+};
+
+__device__ __forceinline__ int tiles_of(const Matrix &m, int phase) {
+    const int n = (int)min(m.rows, m.cols), tn = (n + 127) / 128;
+    return phase % 3 < 2 ? tn * (tn + 1) / 2 : tn * (((int)max(m.rows, m.cols) + 127) / 128);
+}
+
+// One warp.
+__device__ __forceinline__ void make_plan(const Group &g, int phase, Plan *plan) {
+    const int lane = threadIdx.x % 32;
+    int tiles = 0, steps = 0;
+    if (lane < g.n) {
+        const Matrix &m = g.m[lane];
+        tiles = tiles_of(m, phase);
+        steps = ((int)(phase % 3 == 0 ? max(m.rows, m.cols) : min(m.rows, m.cols)) + 63) / 64;
+    }
+    int sum = tiles;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += up;
+    }
+    if (lane < g.n) plan->first[lane] = sum - tiles;
+    const int items = __shfl_sync(0xffffffffu, sum, 31);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) steps = max(steps, __shfl_xor_sync(0xffffffffu, steps, o));
+    if (lane == 0) {
+        plan->items = items;
+        plan->first[g.n] = items;
+        // Slices while every slice finds an SM at once and has a step to take.
+        int splits = 1;
+        while (splits < 8 && 2 * splits * items <= (int)gridDim.x && 2 * splits <= steps) splits *= 2;
+        plan->splits = splits;
+    }
+}
+
+struct Item {
+    int matrix, m0, n0, k0, k1;
+    bool mirror;
+};
+
+__device__ __forceinline__ Item find_item(const Group &g, const Plan &plan, int w, int phase) {
+    Item it;
+    const int item = w / plan.splits, slice = w - item * plan.splits;
+    int i = 0;
+    while (plan.first[i + 1] <= item) ++i;
+    const Matrix &m = g.m[i];
+    const int n = (int)min(m.rows, m.cols), tn = (n + 127) / 128;
+    int t = item - plan.first[i], bi, bj;
+    if (phase % 3 < 2) {
+        bi = 0;
+        for (int left = tn; t >= left; --left) {
+            t -= left;
+            ++bi;
+        }
+        bj = bi + t;
+        it.mirror = bj > bi;
+    } else {
+        bj = t / tn;
+        bi = t - bj * tn;
+        it.mirror = false;
+    }
+    const int steps = ((int)(phase % 3 == 0 ? max(m.rows, m.cols) : min(m.rows, m.cols)) + 63) / 64;
+    const int per = (steps + plan.splits - 1) / plan.splits;
+    it.matrix = i;
+    it.m0 = bi * 128;
+    it.n0 = bj * 128;
+    it.k0 = min(steps, slice * per);
+    it.k1 = min(steps, it.k0 + per);
+    return it;
+}
+
+// Instruction descriptor: f16 operands, f32 sums.
+__host__ __device__ constexpr uint32_t half_idesc(bool q_mn, int m, int n) {
+    return make_idesc(false, q_mn, m, n) & ~((7u << 7) | (7u << 10));
+}
+
+// What one CTA wrote, in generic accesses, is read by any CTA after the barrier, by TMA too.  Every wait is bounded; false
+// once a wait has given up, here or in another CTA.
+__device__ __forceinline__ bool grid_sync(int *arrived, int target, int *status, volatile int *abort_flag) {
+    asm volatile("fence.proxy.async;" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        __threadfence();
+        atomicAdd(arrived, 1);
+        uint64_t t0 = 0;
+        for (uint32_t it = 0;; ++it) {
+            int seen;
+            asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(seen) : "l"(arrived) : "memory");
+            if (seen >= target) break;
+            if ((it & 255u) == 255u) {
+                const uint64_t now = global_timer_ns();
+                if (t0 == 0) t0 = now;
+                if (*abort_flag || now - t0 > 2000000000ull || *reinterpret_cast<volatile int *>(status) != 0) {
+                    atomicCAS(status, 0, 205);
+                    *abort_flag = 1;
+                    break;
+                }
+            }
+        }
+        __threadfence();
+    }
+    __syncthreads();
+    asm volatile("fence.proxy.async;" ::: "memory");
+    return *abort_flag == 0;
+}
+
+// counters: [0] arrivals at the grid's barrier, [1] CTAs that have left, [2 ...] slices of a tile that are done; zero before
+// and after.  sums: a tile's slices as f32, [item][slice][128][128].
+template <class T>
+__global__ void __launch_bounds__(kThreads, 1)
+    muon_kernel(const __grid_constant__ CUtensorMap map, __half *planes, double *parts, float *sums, int *counters, int *status,
+                const __grid_constant__ Group g) {
+    constexpr bool BF16 = sizeof(T) == 2;
+    // 64-k steps that one accumulator adds: tcgen05 cuts its sums off rather than rounding them, by up to 2^-23 of the sum
+    // so far an addition
+    constexpr int kAccStages = BF16 ? 16 : 1;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + kStages * kStage);
+    uint64_t *full = bars, *empty = bars + kStages, *acc_full = bars + 2 * kStages, *acc_empty = acc_full + 2;
+    uint32_t *slot = reinterpret_cast<uint32_t *>(acc_empty + 2);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(slot + 1);
+    int *last_slice = reinterpret_cast<int *>(slot + 2);
+    Plan *plan = reinterpret_cast<Plan *>(slot + 4);
+    double *scratch = reinterpret_cast<double *>(bars + 40);
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+
+    if (threadIdx.x == 0) {
+        prefetch_tmap(&map);
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(smem_u32(&full[s]), 1);
+            mbar_init(smem_u32(&empty[s]), 1);
+        }
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(smem_u32(&acc_full[s]), 1);
+            mbar_init(smem_u32(&acc_empty[s]), kEpiWarps);
+        }
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 1) {
+        tmem_alloc(smem_u32(slot), 256);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *slot;
+    int barriers = 0;
+    bool ok = true;
+
+    if (g.inside) {
+        for (int w = blockIdx.x, i = 0, before = 0; i < g.n; before += g.m[i].parts, ++i)
+            for (; w < before + g.m[i].parts; w += gridDim.x) momentum_part<T>(g.m[i], g.rule, w - before, parts, scratch);
+        ok = grid_sync(counters, ++barriers * gridDim.x, status, abort_flag);
+        for (int w = blockIdx.x, i = 0, before = 0; ok && i < g.n; ++i) {
+            const int blocks = g.m[i].x.plane / 64;
+            if (w < before + blocks) {
+                const double inv = inverse_norm(g.m[i], parts, scratch);
+                for (; w < before + blocks; w += gridDim.x)
+                    split_tile<T>(g.m[i], g.rule, w - before, inv, planes, reinterpret_cast<float(*)[65]>(smem));
+            }
+            before += blocks;
+        }
+        ok = ok && grid_sync(counters, ++barriers * gridDim.x, status, abort_flag);
+    }
+
+    // Stages taken so far, and accumulators: the place in the rings and the parity of their barriers.
+    int stages = 0, accs = 0;
+    for (int phase = 0; ok && phase < 3 * g.steps; ++phase) {
+        if (warp == 0) make_plan(g, phase, plan);
+        __syncthreads();
+        const int units = plan->items * plan->splits, splits = plan->splits;
+        if (warp == 0) {
+            for (int w = blockIdx.x; w < units; w += gridDim.x) {
+                const Item it = find_item(g, *plan, w, phase);
+                const Job j = make_job<T>(g.m[it.matrix], phase, g.steps);
+                const int per = j.planes == 2 ? 1 : 2, count = (it.k1 - it.k0 + per - 1) / per;
+                if (elect_one()) {
+                    for (int c = 0; c < count; ++c) {
+                        const int at_stage = (stages + c) % kStages, round = (stages + c) / kStages;
+                        if (!mbar_wait(smem_u32(&empty[at_stage]), (round & 1) ^ 1, abort_flag)) {
+                            atomicCAS(status, 0, 201);
+                            break;
+                        }
+                        const uint32_t bar = smem_u32(&full[at_stage]), dst = smem_u32(smem + at_stage * kStage);
+                        const int k = it.k0 + c * per, halves = j.planes == 2 || k + 1 < it.k1 ? 2 : 1;
+                        mbar_arrive_expect_tx(bar, halves * kHalf);
+                        for (int h = 0; h < halves; ++h) {
+                            const int pl = j.planes == 2 ? h : 0, kk = j.planes == 2 ? k : k + h;
+                            const int p_row = j.p.row + pl * j.p.plane + kk * j.p.rp + it.m0;
+                            const int q_row = j.q.row + pl * j.q.plane + (j.q_mn ? it.n0 / 64 * j.q.rp + kk * 64 : kk * j.q.rp + it.n0);
+                            const uint32_t to = dst + h * kHalf;
+                            tma_load_2d(to, &map, bar, 0, p_row);
+                            tma_load_2d(to + kBox, &map, bar, 0, p_row + 64);
+                            tma_load_2d(to + 2 * kBox, &map, bar, 0, q_row);
+                            tma_load_2d(to + 3 * kBox, &map, bar, 0, q_row + (j.q_mn ? j.q.rp : 64));
+                        }
+                    }
+                }
+                __syncwarp();
+                stages += count;
+            }
+        } else if (warp == 1) {
+            for (int w = blockIdx.x; w < units; w += gridDim.x) {
+                const Item it = find_item(g, *plan, w, phase);
+                const Job j = make_job<T>(g.m[it.matrix], phase, g.steps);
+                const int per = j.planes == 2 ? 1 : 2, count = (it.k1 - it.k0 + per - 1) / per;
+                if (elect_one()) {
+                    const uint32_t idesc = half_idesc(j.q_mn, 128, 128);
+                    const uint32_t q_step = j.q_mn ? 16 * 128 : 32, q_lbo = j.q_mn ? kBox : 0;
+                    for (int c = 0; c < count; ++c) {
+                        const int acc = accs + c / kAccStages;
+                        if (c % kAccStages == 0 && !mbar_wait(smem_u32(&acc_empty[acc % 2]), (acc / 2 & 1) ^ 1, abort_flag)) {
+                            atomicCAS(status, 0, 202);
+                            break;
+                        }
+                        const int at_stage = (stages + c) % kStages;
+                        if (!mbar_wait(smem_u32(&full[at_stage]), (stages + c) / kStages & 1, abort_flag)) {
+                            atomicCAS(status, 0, 203);
+                            break;
+                        }
+                        tc_fence_after();
+                        const uint32_t d = tmem + acc % 2 * 128, base = smem_u32(smem + at_stage * kStage);
+                        auto mma = [&](int hp, int hq, int i, bool add) {
+                            umma_bf16(d, make_smem_desc(base + hp * kHalf + i * 32, 0, 1024),
+                                      make_smem_desc(base + hq * kHalf + 2 * kBox + i * q_step, q_lbo, 1024), idesc, add ? 1u : 0u);
+                        };
+                        const bool more = c % kAccStages != 0;
+                        if (j.planes == 2) {
+                            // the small products first: what an addition cuts off is a part of the sum so far
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                mma(0, 1, i, more || i > 0);
+                                mma(1, 0, i, true);
+                            }
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) mma(0, 0, i, true);
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) mma(0, 0, i, more || i > 0);
+                            if (it.k0 + 2 * c + 1 < it.k1)
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) mma(1, 1, i, true);
+                        }
+                        umma_commit(smem_u32(&empty[at_stage]));
+                        if ((c + 1) % kAccStages == 0 || c + 1 == count) umma_commit(smem_u32(&acc_full[acc % 2]));
+                    }
+                }
+                __syncwarp();
+                stages += count;
+                accs += (count + kAccStages - 1) / kAccStages;
+            }
+        } else {
+            const int quarter = warp % 4, half = (warp - 2) / 4, row = quarter * 32 + lane;
+            for (int w = blockIdx.x; w < units; w += gridDim.x) {
+                const Item it = find_item(g, *plan, w, phase);
+                const Matrix &m = g.m[it.matrix];
+                const Job j = make_job<T>(m, phase, g.steps);
+                const int per = j.planes == 2 ? 1 : 2, count = (it.k1 - it.k0 + per - 1) / per;
+                float sum[64];
+#pragma unroll
+                for (int c = 0; c < 64; ++c) sum[c] = 0.f;
+                const int reads = (count + kAccStages - 1) / kAccStages;
+                for (int c = 0; c < reads; ++c) {
+                    const int acc = accs + c;
+                    if (!mbar_wait(smem_u32(&acc_full[acc % 2]), acc / 2 & 1, abort_flag)) {
+                        if (lane == 0) atomicCAS(status, 0, 204);
+                        break;
+                    }
+                    __syncwarp();
+                    tc_fence_after();
+                    const uint32_t t = tmem + acc % 2 * 128 + half * 64 + ((uint32_t)(quarter * 32) << 16);
+#pragma unroll
+                    for (int b = 0; b < 64; b += 32) {
+                        uint32_t v[32];
+                        tmem_ld_32x32(t + b, v);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) sum[b + i] += __uint_as_float(v[i]);
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_u32(&acc_empty[acc % 2]));
+                }
+                accs += reads;
+                __syncwarp();
+                if (*abort_flag) break;
+                if (splits > 1) {
+                    // The slice that is done last adds the others', in their order, and goes on.
+                    const int item = w / splits;
+                    float *mine = sums + ((int64_t)w * 128 + row) * 128 + half * 64;
+#pragma unroll
+                    for (int c = 0; c < 64; c += 4)
+                        __stcg(reinterpret_cast<float4 *>(mine + c), make_float4(sum[c], sum[c + 1], sum[c + 2], sum[c + 3]));
+                    __threadfence();
+                    asm volatile("bar.sync 1, %0;" ::"n"(kEpiWarps * 32) : "memory");
+                    if (threadIdx.x == 64) {
+                        const int n = atomicAdd(counters + 2 + item, 1);
+                        if (n == splits - 1) counters[2 + item] = 0;
+                        *last_slice = n == splits - 1;
+                        __threadfence();
+                    }
+                    asm volatile("bar.sync 1, %0;" ::"n"(kEpiWarps * 32) : "memory");
+                    const bool mine_last = *last_slice;
+                    asm volatile("bar.sync 1, %0;" ::"n"(kEpiWarps * 32) : "memory");
+                    if (!mine_last) continue;
+#pragma unroll
+                    for (int c = 0; c < 64; c += 8) {
+                        float v[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) v[i] = 0.f;
+                        for (int z = 0; z < splits; ++z) {
+                            const float *from = sums + (((int64_t)item * splits + z) * 128 + row) * 128 + half * 64 + c;
+                            const float4 lo = __ldcg(reinterpret_cast<const float4 *>(from));
+                            const float4 hi = __ldcg(reinterpret_cast<const float4 *>(from + 4));
+                            v[0] += lo.x; v[1] += lo.y; v[2] += lo.z; v[3] += lo.w;
+                            v[4] += hi.x; v[5] += hi.y; v[6] += hi.z; v[7] += hi.w;
+                        }
+                        finish8<T>(j, m, g.rule, planes, it.m0 + row, it.n0 + half * 64 + c, v, it.mirror);
+                    }
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 64; c += 8) {
+                        float v[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) v[i] = sum[c + i];
+                        finish8<T>(j, m, g.rule, planes, it.m0 + row, it.n0 + half * 64 + c, v, it.mirror);
+                    }
+                }
+                __syncwarp();   // rows beyond the matrix have left finish8 early, and what follows takes whole warps
+            }
+        }
+        if (phase + 1 < 3 * g.steps) ok = grid_sync(counters, ++barriers * gridDim.x, status, abort_flag);
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (*abort_flag) {
+        const uint64_t t0 = global_timer_ns();
+        while (global_timer_ns() - t0 < 200000ull) __nanosleep(1000);
+    }
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 256);
+    }
+    // The last CTA to leave, when all have passed the last barrier, clears the counts for the next launch.
+    if (threadIdx.x == 0) {
+        __threadfence();
+        if (atomicAdd(counters + 1, 1) == (int)gridDim.x - 1) {
+            counters[0] = 0;
+            counters[1] = 0;
+        }
+    }
+}
+
+}  // namespace muon
+}  // namespace ag

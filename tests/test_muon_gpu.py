@@ -90,12 +90,14 @@ def test_large_matrices(dev, rows, cols, seed, dtype):
 
 @gpu
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
-def test_a_list_is_its_matrices(dev, dtype):
-    """Matrices of all sizes in one call have the bits that they have alone."""
+def test_a_list_of_matrices(dev, dtype):
+    """Matrices of all sizes in one call.  How many thread blocks share a matrix goes by the whole call, and the order of its
+    sums with it: the same call has the same bits again, a matrix alone has those of its own call."""
     gs = [_gradient(r, c, i).to(dtype).to(dev.torch_device) for i, (r, c) in enumerate(SIZES)]
     together = dev.newton_schulz(gs)
-    for g, o in zip(gs, together):
-        assert torch.equal(o, dev.newton_schulz([g])[0]), tuple(g.shape)
+    for g, o, again in zip(gs, together, dev.newton_schulz(gs)):
+        assert torch.equal(o, again)
+        _close(o, _polar64(g), dtype)
     many = [_rand((3, 5), i).to(dtype).to(dev.torch_device) for i in range(100)]
     for g, o in zip(many, dev.newton_schulz(many)):
         _close(o, _polar64(g), dtype)
@@ -144,12 +146,13 @@ def test_zeros_and_values_that_are_not_finite(dev, rows, cols, dtype):
     zero = torch.zeros((rows, cols), dtype=dtype, device=dev.torch_device)
     assert not dev.newton_schulz([zero])[0].any()
     good = _gradient(50, 70, 3).to(dtype).to(dev.torch_device)
-    alone, = dev.newton_schulz([good])
+    clean = dev.newton_schulz([good, _gradient(rows, cols, 1).to(dtype).to(dev.torch_device), zero])
+    _close(clean[0], _polar64(good), dtype)
     for bad in (float("nan"), float("inf"), -float("inf")):
         g = _gradient(rows, cols, 1).to(dtype).to(dev.torch_device)
         g[rows // 2, cols - 1] = bad
         o = dev.newton_schulz([good, g, zero])
-        assert torch.equal(o[0], alone) and o[1].isnan().all() and not o[2].any()
+        assert torch.equal(o[0], clean[0]) and o[1].isnan().all() and not o[2].any()
 
 
 @gpu
