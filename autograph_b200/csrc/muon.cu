@@ -55,6 +55,27 @@ struct Space {
     }
 };
 
+template <class T, int BN>
+static int launch(ag_device *dev, const CUtensorMap &map, __half *planes, double *norms, float4 *slices, const Group &g) {
+    auto kernel = muon_kernel<T, BN>;
+    static SmemAllowed allowed;
+    AG_TRY(allow_smem<kSmem>(dev, kernel, allowed));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)dev->sm_count);
+    cfg.blockDim = kThreads;
+    cfg.dynamicSmemBytes = kSmem;
+    cfg.stream = dev->stream;
+    // the grid's barrier needs all CTAs at once
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeCooperative;
+    attr.val.cooperative = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    AG_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, map, planes, norms, slices, dev->tile_counters, dev->status_dev, g));
+    AG_CHECK_LAUNCH();
+    return AG_OK;
+}
+
 template <class T>
 int run(ag_device *dev, const std::vector<Matrix> &matrices, const Rule &rule, int steps) {
     for (size_t first = 0; first < matrices.size(); first += kGroup) {
@@ -64,7 +85,7 @@ int run(ag_device *dev, const std::vector<Matrix> &matrices, const Rule &rule, i
         g.rule = rule;
         Space space;
         int parts = 0, blocks = 0;
-        int64_t values = 0;
+        int64_t values = 0, tiles = 0;
         for (int i = 0; i < g.n; ++i) {
             Matrix &m = g.m[i];
             m = matrices[first + i];
@@ -78,14 +99,16 @@ int run(ag_device *dev, const std::vector<Matrix> &matrices, const Rule &rule, i
             parts += m.parts;
             blocks += m.x.plane / 64;
             values += n * wide;
+            tiles += ceil_div(n, 128) * ceil_div(wide, 128);
         }
         AG_REQUIRE(space.rows < (1ll << 31), AG_ERR_LIMIT, "newton_schulz: the matrices' workspace is too large");
         g.inside = values <= kInside;
+        const bool narrow = tiles <= dev->sm_count;
         const size_t heads = (size_t)kGroup * kMostParts * sizeof(double), sums = (size_t)dev->sm_count * 128 * 128 * sizeof(float);
         void *ws;
         AG_TRY(engine_scratch(dev, heads + sums + (size_t)space.rows * 128, &ws));
         double *norms = (double *)ws;
-        float *slices = (float *)((char *)ws + heads);
+        float4 *slices = (float4 *)((char *)ws + heads);
         __half *planes = (__half *)((char *)ws + heads + sums);
         CUtensorMap map;
         const uint64_t dims[2] = {64, (uint64_t)space.rows}, strides[1] = {64};
@@ -97,22 +120,7 @@ int run(ag_device *dev, const std::vector<Matrix> &matrices, const Rule &rule, i
             split_kernel<T><<<blocks, 256, 0, dev->stream>>>(g, norms, planes);
             AG_CHECK_LAUNCH();
         }
-        auto kernel = muon_kernel<T>;
-        static SmemAllowed allowed;
-        AG_TRY(allow_smem<kSmem>(dev, kernel, allowed));
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3((unsigned)dev->sm_count);
-        cfg.blockDim = kThreads;
-        cfg.dynamicSmemBytes = kSmem;
-        cfg.stream = dev->stream;
-        // the grid's barrier needs all CTAs at once
-        cudaLaunchAttribute attr;
-        attr.id = cudaLaunchAttributeCooperative;
-        attr.val.cooperative = 1;
-        cfg.attrs = &attr;
-        cfg.numAttrs = 1;
-        AG_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, map, planes, norms, slices, dev->tile_counters, dev->status_dev, g));
-        AG_CHECK_LAUNCH();
+        AG_TRY((narrow ? launch<T, 64>(dev, map, planes, norms, slices, g) : launch<T, 128>(dev, map, planes, norms, slices, g)));
     }
     return AG_OK;
 }

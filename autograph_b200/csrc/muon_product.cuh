@@ -98,54 +98,113 @@ __device__ __forceinline__ void join8(const uint4 &hi, const uint4 &lo, float (&
     }
 }
 
-// o = x, or w = (1 - lr * decay) * w - lr * scale * x.
+// Eight neighbouring values of a row of the result from x: o = x, or w = (1 - lr * decay) * w - lr * scale * x.
 template <class T>
-__device__ __forceinline__ void store_final(const Matrix &m, const Rule &r, int M, int N, int row, int col, const float (&v)[8]) {
+__device__ __forceinline__ void store_final(const Matrix &m, const Rule &r, int M, int N, int row, int col, const float (&x)[8]) {
+    if (row >= M || col >= N) return;
     T *o = reinterpret_cast<T *>(m.o);
-    if (row >= M) return;
-    const bool flip = m.rows > m.cols, update = m.v != nullptr;
+    const bool update = m.v != nullptr;
     const float keep = 1.f - r.lr * r.decay, step = -r.lr * m.scale;
+    if (m.rows > m.cols) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-        if (col + i < N) {
-            T *p = flip ? o + (int64_t)(col + i) * m.cols + row : o + (int64_t)row * m.cols + col + i;
-            *p = from_f32<T>(update ? fmaf(step, v[i], keep * to_f32(*p)) : v[i]);
-        }
-}
-
-// Columns col .. col + 7 (col a multiple of 8) of a row of D from their sums.  `mirror`: also the transposed place.
-// What another SM has stored in this launch is read past the SM's own cache.
-template <class T>
-__device__ __forceinline__ void finish8(const Job &j, const Matrix &m, const Rule &r, __half *planes, int row, int col,
-                                        float (&v)[8], bool mirror) {
-    if (row >= (j.M + 127) / 128 * 128 || col >= (j.N + 63) / 64 * 64) return;
-    if (j.has_e) {
-        const int64_t i = at(j.e, row, col);
-        float e[8];
-        join8(__ldcg(reinterpret_cast<const uint4 *>(planes + i)),
-              __ldcg(reinterpret_cast<const uint4 *>(planes + i + (int64_t)j.e.plane * 64)), e);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = fmaf(j.c0, v[k], j.c1 * e[k]);
-    } else {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] *= j.c0;
-    }
-    if (j.final) {
-        store_final<T>(m, r, j.M, j.N, row, col, v);
+        for (int i = 0; i < 8; ++i)
+            if (col + i < N) {
+                T *p = o + (int64_t)(col + i) * m.cols + row;
+                *p = from_f32<T>(update ? fmaf(step, x[i], keep * to_f32(*p)) : x[i]);
+            }
         return;
     }
-    uint4 hi, lo;
-    split8(v, hi, lo);
-    const int64_t i = at(j.d, row, col), plane = (int64_t)j.d.plane * 64;
-    *reinterpret_cast<uint4 *>(planes + i) = hi;
-    *reinterpret_cast<uint4 *>(planes + i + plane) = lo;
-    if (mirror) {
-        const uint32_t h[4] = {hi.x, hi.y, hi.z, hi.w}, l[4] = {lo.x, lo.y, lo.z, lo.w};
-        unsigned short *m = reinterpret_cast<unsigned short *>(planes) + at(j.d, col, row);
+    T *p = o + (int64_t)row * m.cols + col;
+    constexpr int V = 16 / (int)sizeof(T);
+    if (col + 8 <= N && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            m[k * 64] = (unsigned short)(h[k / 2] >> (k % 2 * 16));
-            m[k * 64 + plane] = (unsigned short)(l[k / 2] >> (k % 2 * 16));
+        for (int b = 0; b < 8; b += V) {
+            union {
+                uint4 raw;
+                T v[V];
+            } w;
+            if (update) w.raw = *reinterpret_cast<const uint4 *>(p + b);
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                w.v[i] = from_f32<T>(update ? fmaf(step, x[b + i], keep * to_f32(w.v[i])) : x[b + i]);
+            *reinterpret_cast<uint4 *>(p + b) = w.raw;
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (col + i < N) p[i] = from_f32<T>(update ? fmaf(step, x[i], keep * to_f32(p[i])) : x[i]);
+}
+
+// Columns col .. col + 31 (col a multiple of 32) of a row of D from their sums, by whole warps whose lanes have neighbouring
+// rows.  `mirror`: also the transposed place.  The addend is loaded before the sums are there; what another SM has stored in
+// this launch is read past the SM's own cache.
+struct Addend {
+    uint4 hi[4], lo[4];
+};
+__device__ __forceinline__ void load_addend(const Job &j, const __half *planes, int row, int col, Addend &a) {
+    if (!j.has_e || row >= (j.M + 127) / 128 * 128 || col >= (j.N + 63) / 64 * 64) return;
+    const uint4 *e = reinterpret_cast<const uint4 *>(planes + at(j.e, row, col));
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+        a.hi[b] = __ldcg(e + b);
+        a.lo[b] = __ldcg(e + b + (int64_t)j.e.plane * 8);
+    }
+}
+template <class T>
+__device__ __forceinline__ void finish32(const Job &j, const Matrix &m, const Rule &r, __half *planes, int row, int col,
+                                         float *v, const Addend &a, bool mirror) {
+    const bool in = row < (j.M + 127) / 128 * 128;
+    const int cols = (j.N + 63) / 64 * 64;
+    if (col >= cols) return;   // 64 columns are all in or all out
+    if (j.has_e) {
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            float e8[8];
+            join8(a.hi[b], a.lo[b], e8);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[8 * b + i] = fmaf(j.c0, v[8 * b + i], j.c1 * e8[i]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] *= j.c0;
+    }
+    if (j.final) {
+#pragma unroll
+        for (int b = 0; b < 32; b += 8) {
+            float x[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = v[b + i];
+            store_final<T>(m, r, j.M, j.N, row, col + b, x);
+        }
+        return;
+    }
+    const int64_t plane = (int64_t)j.d.plane * 64;
+    __half *d = planes + at(j.d, row, col);
+    const int lane = threadIdx.x % 32;
+    // the transposed place of rows row, row + 1: an even lane stores their upper halves, an odd one their lower
+    uint32_t *t = reinterpret_cast<uint32_t *>(planes + at(j.d, col, row & ~1) + (lane & 1 ? plane : 0));
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = v[8 * b + i];
+        uint4 hi, lo;
+        split8(x, hi, lo);
+        if (in) {
+            reinterpret_cast<uint4 *>(d)[b] = hi;
+            reinterpret_cast<uint4 *>(d + plane)[b] = lo;
+        }
+        if (mirror) {
+            const uint32_t h[4] = {hi.x, hi.y, hi.z, hi.w}, l[4] = {lo.x, lo.y, lo.z, lo.w};
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint32_t sel = i % 2 ? 0x7632 : 0x5410;
+                const uint32_t both = __byte_perm(h[i / 2], l[i / 2], sel);   // hi | lo << 16
+                const uint32_t other = __shfl_xor_sync(0xffffffffu, both, 1);
+                const uint32_t pair = lane & 1 ? __byte_perm(other, both, 0x7632) : __byte_perm(both, other, 0x5410);
+                if (in) t[(8 * b + i) * 32] = pair;
+            }
         }
     }
 }
@@ -231,8 +290,8 @@ __device__ __forceinline__ void split_tile(const Matrix &m, const Rule &r, int b
 
 constexpr int kEpiWarps = 8, kThreads = 64 + kEpiWarps * 32;
 constexpr int kBox = 64 * 64 * 2;          // bytes of a box of the tensor map
-constexpr int kHalf = 4 * kBox;            // 128 rows of P and of Q, 64 k, one plane
-constexpr int kStage = 2 * kHalf, kStages = 3;   // both planes of 64 k, or the upper one of 128
+// A stage: both planes of 64 k, or the upper one of 128, of 128 rows of P and up to 128 of Q.
+constexpr int kStage = 8 * kBox, kStages = 3;
 constexpr int kSmem = kStages * kStage + 1024 + 512;
 
 // Products of planes of a step.  bf16 results: the products of the last step and of those before the last three are of the
@@ -289,24 +348,29 @@ __device__ __forceinline__ Job make_job(const Matrix &m, int phase, int steps) {
     return j;
 }
 
-// The work items of a phase: tiles of 128 x 128, of all matrices in a row, each cut in `splits` slices of its depth.
+// The work items of a phase: tiles of 128 x BN, of all matrices in a row, each cut in `splits` slices of its depth.
 struct Plan {
     int items, splits;
     int first[kGroup + 1];   // of each matrix's tiles
 };
 
-__device__ __forceinline__ int tiles_of(const Matrix &m, int phase) {
-    const int n = (int)min(m.rows, m.cols), tn = (n + 127) / 128;
-    return phase % 3 < 2 ? tn * (tn + 1) / 2 : tn * (((int)max(m.rows, m.cols) + 127) / 128);
+// Tiles of a symmetric product: those that touch the diagonal or lie above it.  With tiles narrower than high, a row of
+// tiles starts at the first that reaches its rows.
+template <int BN>
+__device__ __forceinline__ int tiles_of(int n, int wide, bool symmetric) {
+    const int tm = (n + 127) / 128, tn = (wide + BN - 1) / BN;
+    return symmetric ? tm * tn - 128 / BN * (tm * (tm - 1) / 2) : tm * tn;
 }
 
 // One warp.
+template <int BN>
 __device__ __forceinline__ void make_plan(const Group &g, int phase, Plan *plan) {
     const int lane = threadIdx.x % 32;
     int tiles = 0, steps = 0;
     if (lane < g.n) {
         const Matrix &m = g.m[lane];
-        tiles = tiles_of(m, phase);
+        const int n = (int)min(m.rows, m.cols);
+        tiles = tiles_of<BN>(n, phase % 3 < 2 ? n : (int)max(m.rows, m.cols), phase % 3 < 2);
         steps = ((int)(phase % 3 == 0 ? max(m.rows, m.cols) : min(m.rows, m.cols)) + 63) / 64;
     }
     int sum = tiles;
@@ -322,9 +386,9 @@ __device__ __forceinline__ void make_plan(const Group &g, int phase, Plan *plan)
     if (lane == 0) {
         plan->items = items;
         plan->first[g.n] = items;
-        // Slices while every slice finds an SM at once and has a step to take.
+        // Slices while every slice finds an SM at once and has eight steps to take.
         int splits = 1;
-        while (splits < 8 && 2 * splits * items <= (int)gridDim.x && 2 * splits <= steps) splits *= 2;
+        while (splits < 8 && 2 * splits * items <= (int)gridDim.x && 16 * splits <= steps) splits *= 2;
         plan->splits = splits;
     }
 }
@@ -334,32 +398,33 @@ struct Item {
     bool mirror;
 };
 
+template <int BN>
 __device__ __forceinline__ Item find_item(const Group &g, const Plan &plan, int w, int phase) {
     Item it;
     const int item = w / plan.splits, slice = w - item * plan.splits;
     int i = 0;
     while (plan.first[i + 1] <= item) ++i;
     const Matrix &m = g.m[i];
-    const int n = (int)min(m.rows, m.cols), tn = (n + 127) / 128;
+    const int n = (int)min(m.rows, m.cols), tm = (n + 127) / 128;
     int t = item - plan.first[i], bi, bj;
     if (phase % 3 < 2) {
         bi = 0;
-        for (int left = tn; t >= left; --left) {
+        for (int left = (n + BN - 1) / BN; t >= left; left -= 128 / BN) {
             t -= left;
             ++bi;
         }
-        bj = bi + t;
-        it.mirror = bj > bi;
+        bj = bi * (128 / BN) + t;
+        it.mirror = bj * BN >= (bi + 1) * 128;
     } else {
-        bj = t / tn;
-        bi = t - bj * tn;
+        bj = t / tm;
+        bi = t - bj * tm;
         it.mirror = false;
     }
     const int steps = ((int)(phase % 3 == 0 ? max(m.rows, m.cols) : min(m.rows, m.cols)) + 63) / 64;
     const int per = (steps + plan.splits - 1) / plan.splits;
     it.matrix = i;
     it.m0 = bi * 128;
-    it.n0 = bj * 128;
+    it.n0 = bj * BN;
     it.k0 = min(steps, slice * per);
     it.k1 = min(steps, it.k0 + per);
     return it;
@@ -370,14 +435,13 @@ __host__ __device__ constexpr uint32_t half_idesc(bool q_mn, int m, int n) {
     return make_idesc(false, q_mn, m, n) & ~((7u << 7) | (7u << 10));
 }
 
-// What one CTA wrote, in generic accesses, is read by any CTA after the barrier, by TMA too.  Every wait is bounded; false
-// once a wait has given up, here or in another CTA.
+// The barrier of the grid, by all threads.  What a CTA wrote before it, in generic accesses, any CTA may read after it, by TMA
+// too.  Every wait is bounded; false once a wait has given up, here or in another CTA.
 __device__ __forceinline__ bool grid_sync(int *arrived, int target, int *status, volatile int *abort_flag) {
     asm volatile("fence.proxy.async;" ::: "memory");
     __syncthreads();
     if (threadIdx.x == 0) {
-        __threadfence();
-        atomicAdd(arrived, 1);
+        asm volatile("red.release.gpu.global.add.s32 [%0], 1;" ::"l"(arrived) : "memory");
         uint64_t t0 = 0;
         for (uint32_t it = 0;; ++it) {
             int seen;
@@ -393,20 +457,21 @@ __device__ __forceinline__ bool grid_sync(int *arrived, int target, int *status,
                 }
             }
         }
-        __threadfence();
+        asm volatile("fence.proxy.async;" ::: "memory");   // this thread issues the loads by TMA
     }
     __syncthreads();
-    asm volatile("fence.proxy.async;" ::: "memory");
     return *abort_flag == 0;
 }
 
 // counters: [0] arrivals at the grid's barrier, [1] CTAs that have left, [2 ...] slices of a tile that are done; zero before
-// and after.  sums: a tile's slices as f32, [item][slice][128][128].
-template <class T>
+// and after.  sums: a tile's slices, [item][slice][four columns][row].
+template <class T, int BN>
 __global__ void __launch_bounds__(kThreads, 1)
-    muon_kernel(const __grid_constant__ CUtensorMap map, __half *planes, double *parts, float *sums, int *counters, int *status,
+    muon_kernel(const __grid_constant__ CUtensorMap map, __half *planes, double *parts, float4 *sums, int *counters, int *status,
                 const __grid_constant__ Group g) {
     constexpr bool BF16 = sizeof(T) == 2;
+    constexpr int COLS = BN / 2, QBOXES = BN / 64;   // of an epilogue warp; of a stage's half
+    constexpr int HALF = (2 + QBOXES) * kBox;
     // 64-k steps that one accumulator adds: tcgen05 cuts its sums off rather than rounding them, by up to 2^-23 of the sum
     // so far an addition
     constexpr int kAccStages = BF16 ? 16 : 1;
@@ -417,8 +482,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t *slot = reinterpret_cast<uint32_t *>(acc_empty + 2);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(slot + 1);
     int *last_slice = reinterpret_cast<int *>(slot + 2);
-    Plan *plan = reinterpret_cast<Plan *>(slot + 4);
-    double *scratch = reinterpret_cast<double *>(bars + 40);
+    Plan *plans = reinterpret_cast<Plan *>(slot + 4);
+    double *scratch = reinterpret_cast<double *>(bars + 48);
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 
     if (threadIdx.x == 0) {
@@ -464,14 +529,28 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     // Stages taken so far, and accumulators: the place in the rings and the parity of their barriers.
     int stages = 0, accs = 0;
+    if (warp == 0) make_plan<BN>(g, 0, plans);
+    __syncthreads();
     for (int phase = 0; ok && phase < 3 * g.steps; ++phase) {
-        if (warp == 0) make_plan(g, phase, plan);
-        __syncthreads();
+        const Plan *plan = plans + phase % 2;
         const int units = plan->items * plan->splits, splits = plan->splits;
+        // Where this CTA's first item lies does not depend on what the others still compute.
+        Item it = {};
+        Job j = {};
+        if ((int)blockIdx.x < units) {
+            it = find_item<BN>(g, *plan, blockIdx.x, phase);
+            j = make_job<T>(g.m[it.matrix], phase, g.steps);
+        }
+        if (phase > 0) {
+            ok = grid_sync(counters, ++barriers * gridDim.x, status, abort_flag);
+            if (!ok) break;
+        }
         if (warp == 0) {
             for (int w = blockIdx.x; w < units; w += gridDim.x) {
-                const Item it = find_item(g, *plan, w, phase);
-                const Job j = make_job<T>(g.m[it.matrix], phase, g.steps);
+                if (w != (int)blockIdx.x) {
+                    it = find_item<BN>(g, *plan, w, phase);
+                    j = make_job<T>(g.m[it.matrix], phase, g.steps);
+                }
                 const int per = j.planes == 2 ? 1 : 2, count = (it.k1 - it.k0 + per - 1) / per;
                 if (elect_one()) {
                     for (int c = 0; c < count; ++c) {
@@ -482,16 +561,17 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                         const uint32_t bar = smem_u32(&full[at_stage]), dst = smem_u32(smem + at_stage * kStage);
                         const int k = it.k0 + c * per, halves = j.planes == 2 || k + 1 < it.k1 ? 2 : 1;
-                        mbar_arrive_expect_tx(bar, halves * kHalf);
+                        mbar_arrive_expect_tx(bar, halves * HALF);
                         for (int h = 0; h < halves; ++h) {
                             const int pl = j.planes == 2 ? h : 0, kk = j.planes == 2 ? k : k + h;
                             const int p_row = j.p.row + pl * j.p.plane + kk * j.p.rp + it.m0;
                             const int q_row = j.q.row + pl * j.q.plane + (j.q_mn ? it.n0 / 64 * j.q.rp + kk * 64 : kk * j.q.rp + it.n0);
-                            const uint32_t to = dst + h * kHalf;
+                            const uint32_t to = dst + h * HALF;
                             tma_load_2d(to, &map, bar, 0, p_row);
                             tma_load_2d(to + kBox, &map, bar, 0, p_row + 64);
-                            tma_load_2d(to + 2 * kBox, &map, bar, 0, q_row);
-                            tma_load_2d(to + 3 * kBox, &map, bar, 0, q_row + (j.q_mn ? j.q.rp : 64));
+#pragma unroll
+                            for (int b = 0; b < QBOXES; ++b)
+                                tma_load_2d(to + (2 + b) * kBox, &map, bar, 0, q_row + b * (j.q_mn ? j.q.rp : 64));
                         }
                     }
                 }
@@ -500,11 +580,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         } else if (warp == 1) {
             for (int w = blockIdx.x; w < units; w += gridDim.x) {
-                const Item it = find_item(g, *plan, w, phase);
-                const Job j = make_job<T>(g.m[it.matrix], phase, g.steps);
+                if (w != (int)blockIdx.x) {
+                    it = find_item<BN>(g, *plan, w, phase);
+                    j = make_job<T>(g.m[it.matrix], phase, g.steps);
+                }
                 const int per = j.planes == 2 ? 1 : 2, count = (it.k1 - it.k0 + per - 1) / per;
                 if (elect_one()) {
-                    const uint32_t idesc = half_idesc(j.q_mn, 128, 128);
+                    const uint32_t idesc = half_idesc(j.q_mn, 128, BN);
                     const uint32_t q_step = j.q_mn ? 16 * 128 : 32, q_lbo = j.q_mn ? kBox : 0;
                     for (int c = 0; c < count; ++c) {
                         const int acc = accs + c / kAccStages;
@@ -520,8 +602,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                         tc_fence_after();
                         const uint32_t d = tmem + acc % 2 * 128, base = smem_u32(smem + at_stage * kStage);
                         auto mma = [&](int hp, int hq, int i, bool add) {
-                            umma_bf16(d, make_smem_desc(base + hp * kHalf + i * 32, 0, 1024),
-                                      make_smem_desc(base + hq * kHalf + 2 * kBox + i * q_step, q_lbo, 1024), idesc, add ? 1u : 0u);
+                            umma_bf16(d, make_smem_desc(base + hp * HALF + i * 32, 0, 1024),
+                                      make_smem_desc(base + hq * HALF + 2 * kBox + i * q_step, q_lbo, 1024), idesc,
+                                      add ? 1u : 0u);
                         };
                         const bool more = c % kAccStages != 0;
                         if (j.planes == 2) {
@@ -549,15 +632,20 @@ __global__ void __launch_bounds__(kThreads, 1)
                 accs += (count + kAccStages - 1) / kAccStages;
             }
         } else {
-            const int quarter = warp % 4, half = (warp - 2) / 4, row = quarter * 32 + lane;
+            const int quarter = warp % 4, half = (warp - 2) / 4, row = quarter * 32 + lane;   // of the tile
             for (int w = blockIdx.x; w < units; w += gridDim.x) {
-                const Item it = find_item(g, *plan, w, phase);
+                if (w != (int)blockIdx.x) {
+                    it = find_item<BN>(g, *plan, w, phase);
+                    j = make_job<T>(g.m[it.matrix], phase, g.steps);
+                }
                 const Matrix &m = g.m[it.matrix];
-                const Job j = make_job<T>(m, phase, g.steps);
+                const int col = it.n0 + half * COLS;
+                Addend e;
+                if (splits == 1) load_addend(j, planes, it.m0 + row, col, e);
                 const int per = j.planes == 2 ? 1 : 2, count = (it.k1 - it.k0 + per - 1) / per;
-                float sum[64];
+                float sum[COLS];
 #pragma unroll
-                for (int c = 0; c < 64; ++c) sum[c] = 0.f;
+                for (int c = 0; c < COLS; ++c) sum[c] = 0.f;
                 const int reads = (count + kAccStages - 1) / kAccStages;
                 for (int c = 0; c < reads; ++c) {
                     const int acc = accs + c;
@@ -567,9 +655,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     __syncwarp();
                     tc_fence_after();
-                    const uint32_t t = tmem + acc % 2 * 128 + half * 64 + ((uint32_t)(quarter * 32) << 16);
+                    const uint32_t t = tmem + acc % 2 * 128 + half * COLS + ((uint32_t)(quarter * 32) << 16);
 #pragma unroll
-                    for (int b = 0; b < 64; b += 32) {
+                    for (int b = 0; b < COLS; b += 32) {
                         uint32_t v[32];
                         tmem_ld_32x32(t + b, v);
                         tmem_ld_wait();
@@ -584,12 +672,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                 __syncwarp();
                 if (*abort_flag) break;
                 if (splits > 1) {
-                    // The slice that is done last adds the others', in their order, and goes on.
+                    // The slice that is done last adds all of them, in their order, and goes on.
                     const int item = w / splits;
-                    float *mine = sums + ((int64_t)w * 128 + row) * 128 + half * 64;
+                    float4 *mine = sums + ((int64_t)w * 32 + half * (COLS / 4)) * 128 + row;
 #pragma unroll
-                    for (int c = 0; c < 64; c += 4)
-                        __stcg(reinterpret_cast<float4 *>(mine + c), make_float4(sum[c], sum[c + 1], sum[c + 2], sum[c + 3]));
+                    for (int c = 0; c < COLS / 4; ++c)
+                        __stcg(mine + c * 128, make_float4(sum[4 * c], sum[4 * c + 1], sum[4 * c + 2], sum[4 * c + 3]));
                     __threadfence();
                     asm volatile("bar.sync 1, %0;" ::"n"(kEpiWarps * 32) : "memory");
                     if (threadIdx.x == 64) {
@@ -602,33 +690,36 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const bool mine_last = *last_slice;
                     asm volatile("bar.sync 1, %0;" ::"n"(kEpiWarps * 32) : "memory");
                     if (!mine_last) continue;
+                    load_addend(j, planes, it.m0 + row, col, e);
 #pragma unroll
-                    for (int c = 0; c < 64; c += 8) {
-                        float v[8];
+                    for (int c = 0; c < COLS; ++c) sum[c] = 0.f;
+                    for (int z = 0; z < splits; ++z) {
+                        const float4 *from = sums + (((int64_t)item * splits + z) * 32 + half * (COLS / 4)) * 128 + row;
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) v[i] = 0.f;
-                        for (int z = 0; z < splits; ++z) {
-                            const float *from = sums + (((int64_t)item * splits + z) * 128 + row) * 128 + half * 64 + c;
-                            const float4 lo = __ldcg(reinterpret_cast<const float4 *>(from));
-                            const float4 hi = __ldcg(reinterpret_cast<const float4 *>(from + 4));
-                            v[0] += lo.x; v[1] += lo.y; v[2] += lo.z; v[3] += lo.w;
-                            v[4] += hi.x; v[5] += hi.y; v[6] += hi.z; v[7] += hi.w;
+                        for (int b = 0; b < COLS / 4; b += 8) {
+                            float4 part[8];
+#pragma unroll
+                            for (int c = 0; c < 8; ++c) part[c] = __ldcg(from + (b + c) * 128);
+#pragma unroll
+                            for (int c = 0; c < 8; ++c) {
+                                sum[4 * (b + c)] += part[c].x;
+                                sum[4 * (b + c) + 1] += part[c].y;
+                                sum[4 * (b + c) + 2] += part[c].z;
+                                sum[4 * (b + c) + 3] += part[c].w;
+                            }
                         }
-                        finish8<T>(j, m, g.rule, planes, it.m0 + row, it.n0 + half * 64 + c, v, it.mirror);
-                    }
-                } else {
-#pragma unroll
-                    for (int c = 0; c < 64; c += 8) {
-                        float v[8];
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) v[i] = sum[c + i];
-                        finish8<T>(j, m, g.rule, planes, it.m0 + row, it.n0 + half * 64 + c, v, it.mirror);
                     }
                 }
-                __syncwarp();   // rows beyond the matrix have left finish8 early, and what follows takes whole warps
+#pragma unroll
+                for (int b = 0; b < COLS / 32; ++b) {
+                    if (b > 0) load_addend(j, planes, it.m0 + row, col + b * 32, e);
+                    finish32<T>(j, m, g.rule, planes, it.m0 + row, col + b * 32, sum + b * 32, e, it.mirror);
+                }
+                __syncwarp();   // rows beyond the matrix leave the last step's stores early, and what follows takes whole warps
             }
         }
-        if (phase + 1 < 3 * g.steps) ok = grid_sync(counters, ++barriers * gridDim.x, status, abort_flag);
+        if (warp == 0 && phase + 1 < 3 * g.steps) make_plan<BN>(g, phase + 1, plans + (phase + 1) % 2);
+        __syncthreads();
     }
 
     tc_fence_before();
