@@ -6,47 +6,173 @@
 //                      dx = rstd * (d - sum d / n - hat * sum(d * hat) / n),
 //                      dweight = sum over rows of dy * hat,  dbias = sum over rows of dy.
 // Everything is computed in f32 and rounded once where it is stored; mean and rstd are f32 tensors.
+//
+// Both directions are bound by memory: forward reads x and writes y, backward reads x and dy and writes dx, once each.  A row
+// is held in registers by a group of G threads (a warp, or a whole CTA), up to 32 values a thread, so that its statistics, and
+// the differences from its mean that the variance is a sum of, cost no second read.  Rows that start on 16 bytes and are
+// whole vectors move 16 bytes a load, others one value, neighbouring lanes on neighbouring values either way.
+// A backward group takes every `groups`-th row and adds dy * hat and dy of its columns in registers as it goes; the CTAs'
+// sums are added in the order of the CTAs, by the CTA that finishes last or, where there is more to add, by a second
+// kernel.  Longer rows take two kernels that read them again.
+//
+// Products that feed a sum are written as __fmul_rn or fmaf: left to the compiler, it fuses them one way in the loop for calls
+// that ask for the statistics, or for one gradient, and another way in the next, and the same values would give other bits.
 #include "common.cuh"
 
 namespace ag {
 namespace norm {
 
-// Sum over the CTA's threads, to all of them; the same order on every run.
-__device__ __forceinline__ float cta_sum(float v, float *scratch) {
+// VEC neighbouring values of T as they lie in memory.
+template <class T, int VEC>
+struct Pack;
+template <>
+struct Pack<float, 4> {
+    float4 v;
+    __device__ __forceinline__ float get(int i) const { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+    __device__ __forceinline__ void set(const float (&x)[4]) { v = make_float4(x[0], x[1], x[2], x[3]); }
+};
+template <>
+struct Pack<__nv_bfloat16, 8> {
+    uint4 v;
+    __device__ __forceinline__ float get(int i) const {
+        const uint32_t w = i / 2 == 0 ? v.x : i / 2 == 1 ? v.y : i / 2 == 2 ? v.z : v.w;
+        return __uint_as_float(i % 2 ? w & 0xffff0000u : w << 16);
+    }
+    __device__ __forceinline__ void set(const float (&x)[8]) {
+        uint32_t w[4];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    const int warp = threadIdx.x / 32, warps = blockDim.x / 32;
-    __syncthreads();
-    if (threadIdx.x % 32 == 0) scratch[warp] = v;
-    __syncthreads();
-    float s = 0.f;
-    for (int i = 0; i < warps; ++i) s += scratch[i];
-    return s;
+        for (int i = 0; i < 4; ++i) {
+            const __nv_bfloat162 p = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+            w[i] = *reinterpret_cast<const uint32_t *>(&p);
+        }
+        v = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+};
+template <class T>
+struct Pack<T, 1> {
+    T v;
+    __device__ __forceinline__ float get(int) const { return to_f32(v); }
+    __device__ __forceinline__ void set(const float (&x)[1]) { v = from_f32<T>(x[0]); }
+};
+
+// Sums over a group's threads, to all of them; the same order on every run.  A group is a warp or the CTA; the CTA's scratch
+// holds N floats a warp.
+template <int G, int N>
+__device__ __forceinline__ void group_sum(float (&v)[N], float *scratch) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+    if constexpr (G > 32) {
+        const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+        __syncthreads();   // the sums before have been read
+        if (lane == 0)
+#pragma unroll
+            for (int i = 0; i < N; ++i) scratch[i * 32 + warp] = v[i];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = lane < G / 32 ? scratch[i * 32 + lane] : 0.f;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+    }
 }
 
-template <class T>
-__global__ void __launch_bounds__(256)
-    layer_norm_kernel(const T *x, const T *weight, const T *bias, int64_t rows, int64_t cols, float eps, T *y, float *mean_out,
+template <int G>
+constexpr int threads_of() { return G == 32 ? 256 : G; }
+
+// Rows in registers: NC packs of VEC values a thread.
+template <class T, int VEC, int G, int NC>
+__global__ void __launch_bounds__(threads_of<G>())
+    layer_norm_kernel(const T *x, const T *weight, const T *bias, int64_t rows, int cols, float eps, T *y, float *mean_out,
                       float *rstd_out) {
-    __shared__ float scratch[8];
+    using P = Pack<T, VEC>;
+    __shared__ float scratch[32];
+    let_dependents_launch();
+    dependency_wait();
+    constexpr int GROUPS = threads_of<G>() / G;
+    const int t = threadIdx.x % G;
+    const float n = (float)cols;
+    for (int64_t row = (int64_t)blockIdx.x * GROUPS + threadIdx.x / G; row < rows; row += (int64_t)gridDim.x * GROUPS) {
+        const T *xr = x + row * cols;
+        P p[NC];
+        float s[1] = {0.f};
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int col = (c * G + t) * VEC;
+            if (col < cols) p[c] = *reinterpret_cast<const P *>(xr + col);
+        }
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+            if ((c * G + t) * VEC < cols)
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) s[0] += p[c].get(i);
+        group_sum<G>(s, scratch);
+        const float mean = __fdiv_rn(s[0], n);   // of equal values, that value
+        s[0] = 0.f;
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+            if ((c * G + t) * VEC < cols)
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    const float d = p[c].get(i) - mean;
+                    s[0] = fmaf(d, d, s[0]);
+                }
+        group_sum<G>(s, scratch);
+        const float rstd = 1.f / sqrtf(__fdiv_rn(s[0], n) + eps);
+        T *yr = y + row * cols;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int col = (c * G + t) * VEC;
+            if (col < cols) {
+                float o[VEC];
+                P w, b;
+                if (weight != nullptr) w = *reinterpret_cast<const P *>(weight + col);
+                if (bias != nullptr) b = *reinterpret_cast<const P *>(bias + col);
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    o[i] = fmaf(__fmul_rn(p[c].get(i) - mean, rstd), weight != nullptr ? w.get(i) : 1.f, bias != nullptr ? b.get(i) : 0.f);
+                }
+                P q;
+                q.set(o);
+                *reinterpret_cast<P *>(yr + col) = q;
+            }
+        }
+        if (t == 0) {
+            if (mean_out != nullptr) mean_out[row] = mean;
+            if (rstd_out != nullptr) rstd_out[row] = rstd;
+        }
+    }
+}
+
+// Rows that no registers hold: read three times.
+template <class T>
+__global__ void __launch_bounds__(1024)
+    layer_norm_long_kernel(const T *x, const T *weight, const T *bias, int64_t rows, int64_t cols, float eps, T *y,
+                           float *mean_out, float *rstd_out) {
+    __shared__ float scratch[32];
     let_dependents_launch();
     dependency_wait();
     for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
         const T *xr = x + row * cols;
-        float s = 0.f;
-        for (int64_t i = threadIdx.x; i < cols; i += 256) s += to_f32(xr[i]);
-        const float mean = cta_sum(s, scratch) / (float)cols;
-        s = 0.f;
-        for (int64_t i = threadIdx.x; i < cols; i += 256) {
+        float s[1] = {0.f};
+#pragma unroll 8
+        for (int64_t i = threadIdx.x; i < cols; i += 1024) s[0] += to_f32(xr[i]);
+        group_sum<1024>(s, scratch);
+        const float mean = s[0] / (float)cols;
+        s[0] = 0.f;
+#pragma unroll 8
+        for (int64_t i = threadIdx.x; i < cols; i += 1024) {
             const float c = to_f32(xr[i]) - mean;
-            s += c * c;
+            s[0] = fmaf(c, c, s[0]);
         }
-        const float rstd = 1.f / sqrtf(cta_sum(s, scratch) / (float)cols + eps);
-        for (int64_t i = threadIdx.x; i < cols; i += 256) {
-            float v = (to_f32(xr[i]) - mean) * rstd;
-            if (weight != nullptr) v *= to_f32(weight[i]);
-            if (bias != nullptr) v += to_f32(bias[i]);
-            y[row * cols + i] = from_f32<T>(v);
+        group_sum<1024>(s, scratch);
+        const float rstd = 1.f / sqrtf(s[0] / (float)cols + eps);
+#pragma unroll 4
+        for (int64_t i = threadIdx.x; i < cols; i += 1024) {
+            const float w = weight != nullptr ? to_f32(weight[i]) : 1.f, b = bias != nullptr ? to_f32(bias[i]) : 0.f;
+            y[row * cols + i] = from_f32<T>(fmaf(__fmul_rn(to_f32(xr[i]) - mean, rstd), w, b));
         }
         if (threadIdx.x == 0) {
             if (mean_out != nullptr) mean_out[row] = mean;
@@ -55,85 +181,336 @@ __global__ void __launch_bounds__(256)
     }
 }
 
+// Where the CTAs' column sums go: partial [CTA][2][cols], added by the CTA that arrives last (arrivals: a zero, and zero
+// again afterwards) or, where that is null, by columns_kernel.
 template <class T>
-__global__ void __launch_bounds__(256)
+struct Columns {
+    float *partial;
+    int *arrivals;
+    float beta;
+    T *dweight, *dbias;
+};
+
+template <class T>
+__device__ __forceinline__ void store_column(const Columns<T> &c, int cols, int i, float s) {
+    T *out = i < cols ? c.dweight : c.dbias;
+    if (out == nullptr) return;
+    out += i < cols ? i : i - cols;
+    *out = from_f32<T>(c.beta != 0.f ? fmaf(c.beta, to_f32(*out), s) : s);
+}
+
+template <class T, int VEC, int G, int NC>
+__global__ void __launch_bounds__(threads_of<G>())
     layer_norm_backward_kernel(const T *x, const T *weight, const float *mean, const float *rstd, const T *dy, int64_t rows,
-                               int64_t cols, T *dx) {
-    __shared__ float scratch[8];
+                               int cols, T *dx, const Columns<T> out) {
+    using P = Pack<T, VEC>;
+    constexpr int THREADS = threads_of<G>(), GROUPS = THREADS / G;
+    // the groups' sums of G == 32, one of the two gradients at a time
+    __shared__ float scratch[G == 32 ? GROUPS * 32 * NC * VEC : 64];
+    __shared__ int last;
+    let_dependents_launch();
+    dependency_wait();
+    const int t = threadIdx.x % G;
+    const float n = (float)cols;
+    float dw[NC * VEC], db[NC * VEC];
+#pragma unroll
+    for (int i = 0; i < NC * VEC; ++i) dw[i] = db[i] = 0.f;
+    for (int64_t row = (int64_t)blockIdx.x * GROUPS + threadIdx.x / G; row < rows; row += (int64_t)gridDim.x * GROUPS) {
+        P px[NC], pd[NC];
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int col = (c * G + t) * VEC;
+            if (col < cols) {
+                px[c] = *reinterpret_cast<const P *>(x + row * cols + col);
+                pd[c] = *reinterpret_cast<const P *>(dy + row * cols + col);
+            }
+        }
+        const float m = mean[row], r = rstd[row];
+        float s[2] = {0.f, 0.f};   // of d, of d * hat
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int col = (c * G + t) * VEC;
+            if (col < cols) {
+                P w;
+                if (weight != nullptr) w = *reinterpret_cast<const P *>(weight + col);
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    const float hat = __fmul_rn(px[c].get(i) - m, r);
+                    float d = pd[c].get(i);
+                    dw[c * VEC + i] = fmaf(d, hat, dw[c * VEC + i]);
+                    db[c * VEC + i] += d;
+                    if (weight != nullptr) d = __fmul_rn(d, w.get(i));
+                    s[0] += d;
+                    s[1] = fmaf(d, hat, s[1]);
+                }
+            }
+        }
+        if (dx == nullptr) continue;
+        group_sum<G>(s, scratch);
+        const float along = __fdiv_rn(s[0], n), across = __fdiv_rn(s[1], n);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int col = (c * G + t) * VEC;
+            if (col < cols) {
+                P w;
+                if (weight != nullptr) w = *reinterpret_cast<const P *>(weight + col);
+                float o[VEC];
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    const float hat = __fmul_rn(px[c].get(i) - m, r);
+                    float d = pd[c].get(i);
+                    if (weight != nullptr) d = __fmul_rn(d, w.get(i));
+                    o[i] = r * fmaf(-hat, across, d - along);
+                }
+                P q;
+                q.set(o);
+                *reinterpret_cast<P *>(dx + row * cols + col) = q;
+            }
+        }
+    }
+    if (out.partial == nullptr) return;
+    float *mine = out.partial + (int64_t)blockIdx.x * 2 * cols;
+    if constexpr (G == 32) {
+        // the CTA's warps, in order
+        const int warp = threadIdx.x / 32;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < NC * VEC; ++i) scratch[(warp * NC * VEC + i) * 32 + t] = half == 0 ? dw[i] : db[i];
+            __syncthreads();
+            for (int k = threadIdx.x; k < NC * VEC * 32; k += THREADS) {
+                const int i = k / 32, lane = k % 32, col = (i / VEC * 32 + lane) * VEC + i % VEC;
+                float s = 0.f;
+#pragma unroll
+                for (int w = 0; w < GROUPS; ++w) s += scratch[w * NC * VEC * 32 + k];
+                if (col < cols) __stcg(mine + half * cols + col, s);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                const int col = (c * G + t) * VEC + i;
+                if (col < cols) {
+                    __stcg(mine + col, dw[c * VEC + i]);
+                    __stcg(mine + cols + col, db[c * VEC + i]);
+                }
+            }
+    }
+    if (out.arrivals == nullptr) return;
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        last = atomicAdd(out.arrivals, 1) == (int)gridDim.x - 1;
+        if (last) *out.arrivals = 0;
+        __threadfence();
+    }
+    __syncthreads();
+    if (!last) return;
+    for (int i = threadIdx.x; i < 2 * cols; i += THREADS) {
+        float s = 0.f;
+#pragma unroll 8
+        for (int k = 0; k < (int)gridDim.x; ++k) s += __ldcg(out.partial + (int64_t)k * 2 * cols + i);
+        store_column(out, cols, i, s);
+    }
+}
+
+// The sums of `parts` CTAs: a CTA takes 32 columns of [2][cols], a warp every eighth part; a part-less call writes beta times
+// what there was.
+template <class T>
+__global__ void __launch_bounds__(256) columns_kernel(int parts, int cols, const Columns<T> out) {
+    __shared__ float sums[8][33];
+    let_dependents_launch();
+    dependency_wait();
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    const int64_t i = (int64_t)blockIdx.x * 32 + lane;
+    float s = 0.f;
+    if (i < 2 * (int64_t)cols)
+#pragma unroll 8
+        for (int k = warp; k < parts; k += 8) s += out.partial[(int64_t)k * 2 * cols + i];
+    sums[warp][lane] = s;
+    __syncthreads();
+    if (warp == 0 && i < 2 * (int64_t)cols) {
+        s = 0.f;
+        for (int w = 0; w < 8; ++w) s += sums[w][lane];
+        store_column(out, cols, (int)i, s);
+    }
+}
+
+template <class T>
+__global__ void __launch_bounds__(1024)
+    layer_norm_long_backward_kernel(const T *x, const T *weight, const float *mean, const float *rstd, const T *dy, int64_t rows,
+                                    int64_t cols, T *dx) {
+    __shared__ float scratch[64];
     let_dependents_launch();
     dependency_wait();
     for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
         const T *xr = x + row * cols, *dr = dy + row * cols;
         const float m = mean[row], r = rstd[row];
-        float along = 0.f, across = 0.f;
-        for (int64_t i = threadIdx.x; i < cols; i += 256) {
-            const float hat = (to_f32(xr[i]) - m) * r;
+        float s[2] = {0.f, 0.f};
+#pragma unroll 4
+        for (int64_t i = threadIdx.x; i < cols; i += 1024) {
+            const float hat = __fmul_rn(to_f32(xr[i]) - m, r);
             float d = to_f32(dr[i]);
-            if (weight != nullptr) d *= to_f32(weight[i]);
-            along += d;
-            across += d * hat;
+            if (weight != nullptr) d = __fmul_rn(d, to_f32(weight[i]));
+            s[0] += d;
+            s[1] = fmaf(d, hat, s[1]);
         }
-        along = cta_sum(along, scratch) / (float)cols;
-        across = cta_sum(across, scratch) / (float)cols;
-        for (int64_t i = threadIdx.x; i < cols; i += 256) {
-            const float hat = (to_f32(xr[i]) - m) * r;
+        group_sum<1024>(s, scratch);
+        const float along = s[0] / (float)cols, across = s[1] / (float)cols;
+#pragma unroll 4
+        for (int64_t i = threadIdx.x; i < cols; i += 1024) {
+            const float hat = __fmul_rn(to_f32(xr[i]) - m, r);
             float d = to_f32(dr[i]);
-            if (weight != nullptr) d *= to_f32(weight[i]);
-            dx[row * cols + i] = from_f32<T>(r * (d - along - hat * across));
+            if (weight != nullptr) d = __fmul_rn(d, to_f32(weight[i]));
+            dx[row * cols + i] = from_f32<T>(r * fmaf(-hat, across, d - along));
         }
     }
 }
 
-// A column's sums over all rows: a CTA takes 32 columns, its warps every eighth row.
+// Column sums of long rows: a CTA takes 256 columns and one of gridDim.y slices of the rows.
 template <class T>
 __global__ void __launch_bounds__(256)
-    layer_norm_columns_kernel(const T *x, const float *mean, const float *rstd, const T *dy, int64_t rows, int64_t cols,
-                              float beta, T *dweight, T *dbias) {
-    __shared__ float sums[2][8][33];
+    layer_norm_long_columns_kernel(const T *x, const float *mean, const float *rstd, const T *dy, int64_t rows, int64_t cols,
+                                   float *partial) {
     let_dependents_launch();
     dependency_wait();
-    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-    for (int64_t c0 = (int64_t)blockIdx.x * 32; c0 < cols; c0 += (int64_t)gridDim.x * 32) {
-        const int64_t c = c0 + lane;
-        float w = 0.f, b = 0.f;
-        if (c < cols)
-            for (int64_t r = warp; r < rows; r += 8) {
-                const float d = to_f32(dy[r * cols + c]);
-                w += d * ((to_f32(x[r * cols + c]) - mean[r]) * rstd[r]);
-                b += d;
-            }
-        sums[0][warp][lane] = w;
-        sums[1][warp][lane] = b;
-        __syncthreads();
-        if (warp < 2 && c < cols) {
-            T *out = warp == 0 ? dweight : dbias;
-            float s = 0.f;
-            for (int i = 0; i < 8; ++i) s += sums[warp][i][lane];
-            if (out != nullptr) out[c] = from_f32<T>(beta != 0.f ? beta * to_f32(out[c]) + s : s);
-        }
-        __syncthreads();
+    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (c >= cols) return;
+    float w = 0.f, b = 0.f;
+#pragma unroll 8
+    for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
+        const float d = to_f32(dy[r * cols + c]);
+        w = fmaf(d, (to_f32(x[r * cols + c]) - mean[r]) * rstd[r], w);
+        b += d;
     }
+    partial[(int64_t)blockIdx.y * 2 * cols + c] = w;
+    partial[(int64_t)blockIdx.y * 2 * cols + cols + c] = b;
+}
+
+// ---- host ------------------------------------------------------------------------------------------
+
+template <class T>
+struct Forward {
+    ag_device *dev;
+    const T *x, *weight, *bias;
+    int64_t rows, cols;
+    float eps;
+    T *y;
+    float *mean, *rstd;
+    template <int VEC, int G, int NC>
+    int run() const {
+        constexpr int GROUPS = threads_of<G>() / G;
+        const int64_t blocks = ceil_div(rows, GROUPS), most = (int64_t)dev->sm_count * (2048 / threads_of<G>());
+        return launch_dependent(dev, layer_norm_kernel<T, VEC, G, NC>, dim3((unsigned)(blocks < most ? blocks : most)),
+                                threads_of<G>(), 0, x, weight, bias, rows, (int)cols, eps, y, mean, rstd);
+    }
+};
+
+template <class T>
+struct Backward {
+    ag_device *dev;
+    const T *x, *weight;
+    const float *mean, *rstd;
+    const T *dy;
+    int64_t rows, cols;
+    T *dx;
+    float beta;
+    T *dweight, *dbias;
+    bool sums() const { return dweight != nullptr || dbias != nullptr; }
+
+    int add_columns(int parts, Columns<T> out) const {
+        return launch_dependent(dev, columns_kernel<T>, dim3((unsigned)ceil_div(2 * cols, 32)), 256, 0, parts, (int)cols, out);
+    }
+    template <int VEC, int G, int NC>
+    int run() const {
+        constexpr int GROUPS = threads_of<G>() / G;
+        auto kernel = layer_norm_backward_kernel<T, VEC, G, NC>;
+        static std::atomic<int> resident{0};   // CTAs of an SM
+        int per_sm = resident.load(std::memory_order_relaxed);
+        if (per_sm == 0) {
+            AG_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads_of<G>(), 0));
+            if (per_sm < 1) per_sm = 1;
+            resident.store(per_sm, std::memory_order_relaxed);
+        }
+        const int64_t most = (int64_t)dev->sm_count * per_sm, blocks = ceil_div(rows, GROUPS);
+        const int grid = (int)(blocks < most ? blocks : most);
+        Columns<T> out = {nullptr, nullptr, beta, dweight, dbias};
+        if (sums()) {
+            void *ws;
+            AG_TRY(workspace(dev, (size_t)grid * 2 * cols * sizeof(float), &ws));
+            out.partial = (float *)ws;
+            if ((int64_t)grid * cols <= kLastAdds) out.arrivals = dev->tile_counters;
+        }
+        AG_TRY(launch_dependent(dev, kernel, dim3((unsigned)grid), threads_of<G>(), 0, x, weight, mean, rstd, dy, rows, (int)cols,
+                                dx, out));
+        return out.partial != nullptr && out.arrivals == nullptr ? add_columns(grid, out) : AG_OK;
+    }
+    static constexpr int64_t kLastAdds = 16384;   // partial sums of each gradient that the last CTA adds
+};
+
+// The kernel whose registers hold a row: values a thread rounded up to a power of two, of a warp up to 1024 columns, then of a
+// CTA.  `MOST`: the most values a thread of a CTA may hold.
+template <int VEC, int MOST, class F>
+int by_columns(const F &f) {
+    const int64_t n = f.cols;
+    if (VEC < 8 && n <= 32 * 4) return f.template run<VEC, 32, 4 / (VEC < 8 ? VEC : 1)>();
+    if (n <= 32 * 8) return f.template run<VEC, 32, 8 / VEC>();
+    if (n <= 32 * 16) return f.template run<VEC, 32, 16 / VEC>();
+    if (n <= 32 * 32) return f.template run<VEC, 32, 32 / VEC>();
+    if (n <= 256 * 8) return f.template run<VEC, 256, 8 / VEC>();
+    if (n <= 256 * 16) return f.template run<VEC, 256, 16 / VEC>();
+    if (n <= 512 * 16) return f.template run<VEC, 512, 16 / VEC>();
+    if constexpr (MOST > 16) {
+        if (n <= 1024 * 16) return f.template run<VEC, 1024, 16 / VEC>();
+        return f.template run<VEC, 1024, 32 / VEC>();
+    }
+    return AG_ERR_UNSUPPORTED;
+}
+
+template <class T>
+bool vectors(int64_t cols, std::initializer_list<const void *> tensors) {
+    if (cols * sizeof(T) % 16 != 0) return false;
+    for (const void *p : tensors)
+        if (reinterpret_cast<uintptr_t>(p) % 16 != 0) return false;   // null is
+    return true;
 }
 
 template <class T>
 int forward(ag_device *dev, const T *x, const T *weight, const T *bias, int64_t rows, int64_t cols, float eps, T *y,
             float *mean, float *rstd) {
     if (rows == 0) return AG_OK;
-    const unsigned grid = (unsigned)(rows < (1 << 20) ? rows : 1 << 20);
-    return launch_dependent(dev, layer_norm_kernel<T>, dim3(grid), 256, 0, x, weight, bias, rows, cols, eps, y, mean, rstd);
+    if (cols > 32768) {
+        const int64_t most = 2 * dev->sm_count;
+        return launch_dependent(dev, layer_norm_long_kernel<T>, dim3((unsigned)(rows < most ? rows : most)), 1024, 0, x, weight, bias,
+                                rows, cols, eps, y, mean, rstd);
+    }
+    const Forward<T> f = {dev, x, weight, bias, rows, cols, eps, y, mean, rstd};
+    return vectors<T>(cols, {x, weight, bias, y}) ? by_columns<16 / sizeof(T), 32>(f) : by_columns<1, 32>(f);
 }
 
 template <class T>
 int backward(ag_device *dev, const T *x, const T *weight, const float *mean, const float *rstd, const T *dy, int64_t rows,
              int64_t cols, T *dx, float beta, T *dweight, T *dbias) {
-    if (rows > 0 && dx != nullptr) {
-        const unsigned grid = (unsigned)(rows < (1 << 20) ? rows : 1 << 20);
-        AG_TRY(launch_dependent(dev, layer_norm_backward_kernel<T>, dim3(grid), 256, 0, x, weight, mean, rstd, dy, rows, cols, dx));
+    const Backward<T> f = {dev, x, weight, mean, rstd, dy, rows, cols, dx, beta, dweight, dbias};
+    if (dx == nullptr && !f.sums()) return AG_OK;
+    if (rows == 0) return f.sums() ? f.add_columns(0, {nullptr, nullptr, beta, dweight, dbias}) : AG_OK;
+    if (cols <= 512 * 16) return vectors<T>(cols, {x, weight, dy, dx}) ? by_columns<16 / sizeof(T), 16>(f) : by_columns<1, 16>(f);
+    if (dx != nullptr) {
+        const int64_t most = 2 * dev->sm_count;
+        AG_TRY(launch_dependent(dev, layer_norm_long_backward_kernel<T>, dim3((unsigned)(rows < most ? rows : most)), 1024, 0, x,
+                                weight, mean, rstd, dy, rows, cols, dx));
     }
-    if (dweight == nullptr && dbias == nullptr) return AG_OK;
-    const int64_t blocks = ceil_div(cols, 32);
-    return launch_dependent(dev, layer_norm_columns_kernel<T>, dim3((unsigned)(blocks < (1 << 20) ? blocks : 1 << 20)), 256, 0,
-                            x, mean, rstd, dy, rows, cols, beta, dweight, dbias);
+    if (!f.sums()) return AG_OK;
+    const int64_t blocks = ceil_div(cols, 256), want = ceil_div((int64_t)8 * dev->sm_count, blocks);
+    const int slices = (int)(want < rows ? want : rows);
+    void *ws;
+    AG_TRY(workspace(dev, (size_t)slices * 2 * cols * sizeof(float), &ws));
+    AG_TRY(launch_dependent(dev, layer_norm_long_columns_kernel<T>, dim3((unsigned)blocks, (unsigned)slices), 256, 0, x, mean, rstd,
+                            dy, rows, cols, (float *)ws));
+    return f.add_columns(slices, {(float *)ws, nullptr, beta, dweight, dbias});
 }
 
 static int check_sizes(ag_dtype dtype, int64_t rows, int64_t cols) {
@@ -141,6 +518,7 @@ static int check_sizes(ag_dtype dtype, int64_t rows, int64_t cols) {
     AG_REQUIRE(rows >= 0, AG_ERR_SHAPE, "layer_norm: negative number of rows");
     AG_REQUIRE(cols > 0, AG_ERR_SHAPE, "layer_norm: a row needs at least one value");
     AG_REQUIRE(rows == 0 || cols <= INT64_MAX / 8 / rows, AG_ERR_SHAPE, "layer_norm: size overflows");
+    AG_REQUIRE(cols < (1 << 30), AG_ERR_LIMIT, "layer_norm: rows of %lld values are beyond the limit", (long long)cols);
     return AG_OK;
 }
 

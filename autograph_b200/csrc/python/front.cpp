@@ -33,8 +33,9 @@
     X(ag_gemm) X(ag_dense_forward) X(ag_conv2_forward) X(ag_conv2_backward_input)                  \
     X(ag_conv2_backward_weight) X(ag_conv2_output_shape) X(ag_max_pool2)                           \
     X(ag_max_pool2_backward_from_input) X(ag_relu) X(ag_relu_backward) X(ag_bias_add)              \
-    X(ag_bias_grad) X(ag_model_infer) X(ag_model_infer_u8) X(ag_model_forward_device)              \
-    X(ag_model_train_step) X(ag_model_train_forward_backward) X(ag_model_apply_update)
+    X(ag_bias_grad) X(ag_layer_norm_forward) X(ag_layer_norm_backward) X(ag_model_infer)           \
+    X(ag_model_infer_u8) X(ag_model_forward_device) X(ag_model_train_step)                         \
+    X(ag_model_train_forward_backward) X(ag_model_apply_update)
 
 #define DECLARE(name) static __typeof__(&name) p_##name;
 FUNCTIONS(DECLARE)
@@ -44,12 +45,12 @@ static PyObject *py_check, *device_context;
 
 enum Method {
     M_DOT, M_GEMM, M_DENSE, M_CONV_FWD, M_CONV_DX, M_CONV_DW, M_POOL, M_POOL_BWD, M_RELU, M_RELU_BWD,
-    M_BIAS_ADD, M_BIAS_GRAD, M_INFER, M_INFER_U8, M_FORWARD, M_TRAIN, M_TRAIN_FB, M_UPDATE, M_COUNT
+    M_BIAS_ADD, M_BIAS_GRAD, M_NORM, M_NORM_KEEP, M_NORM_BWD, M_INFER, M_INFER_U8, M_FORWARD, M_TRAIN, M_TRAIN_FB, M_UPDATE, M_COUNT
 };
 static const char *method_names[M_COUNT] = {
     "dot", "gemm", "dense_forward", "conv2_forward", "conv2_backward_input", "conv2_backward_weight",
     "max_pool2", "max_pool2_backward_from_input", "relu", "relu_backward", "bias_add", "bias_grad",
-    "infer", "infer_u8", "forward_device", "train_step", "train_forward_backward", "apply_update"};
+    "layer_norm", "layer_norm_keep", "layer_norm_backward", "infer", "infer_u8", "forward_device", "train_step", "train_forward_backward", "apply_update"};
 static PyObject *fallbacks[M_COUNT];
 
 typedef struct {
@@ -520,6 +521,86 @@ ENTRY(bias_grad) {
     return finish(st, out);
 }
 
+/* Rows and columns of x normalised over its last `n` dimensions, which are those of each given vector. */
+static int norm_sizes(const View *x, int n, int64_t *rows, int64_t *cols) {
+    if (n < 1 || n > x->ndim || x->dtype == AG_U8) return 0;
+    *rows = *cols = 1;
+    for (int i = 0; i < x->ndim; ++i) *(i < x->ndim - n ? rows : cols) *= x->shape[i];
+    return *cols > 0;
+}
+static int norm_vector(PyObject *o, const View *x, int index, int *n, View *v) {
+    v->p = NULL;
+    if (o == NULL || o == Py_None) return 1;
+    if (!view_of(o, 0, 0, index, v) || v->dtype != x->dtype || v->ndim < 1 || v->ndim > x->ndim) return 0;
+    if (*n != 0 && *n != v->ndim) return 0;
+    *n = v->ndim;
+    for (int i = 0; i < v->ndim; ++i)
+        if (v->shape[i] != x->shape[x->ndim - v->ndim + i]) return 0;
+    return 1;
+}
+
+static PyObject *norm_forward(enum Method m, PyObject *self, PyObject *const *args, Py_ssize_t nargs, PyObject *kwnames) {
+    static const char *const names[] = {"x", "weight", "bias", "eps"};
+    DeviceObject *d = (DeviceObject *)self;
+    PyObject *o[4];
+    View x, w, b;
+    float eps;
+    int n = 0, st;
+    int64_t rows, cols;
+    if (!parse(args, nargs, kwnames, names, 4, 1, o) || !plain(d) || !view_of(o[0], 0, 0, d->index, &x) ||
+        !norm_vector(o[1], &x, d->index, &n, &w) || !norm_vector(o[2], &x, d->index, &n, &b) ||
+        !float_of(o[3], 1e-5, &eps) || !norm_sizes(&x, n ? n : 1, &rows, &cols))
+        FALL_BACK(m);
+    void *y, *mean = NULL, *rstd = NULL;
+    PyObject *out = new_tensor(d, x.dtype, x.ndim, x.shape, &y), *kept[2] = {NULL, NULL};
+    if (out == NULL) return NULL;
+    if (m == M_NORM_KEEP) {
+        const int lead = x.ndim - (n ? n : 1);
+        kept[0] = new_tensor(d, AG_F32, lead, x.shape, &mean);
+        kept[1] = kept[0] ? new_tensor(d, AG_F32, lead, x.shape, &rstd) : NULL;
+        if (kept[1] == NULL) {
+            Py_XDECREF(kept[0]);
+            Py_DECREF(out);
+            return NULL;
+        }
+    }
+    CALL(st, p_ag_layer_norm_forward(d->h, (ag_dtype)x.dtype, x.p, w.p, b.p, rows, cols, eps, y, (float *)mean,
+                                     (float *)rstd));
+    if (m == M_NORM) return finish(st, out);
+    return finish(st, Py_BuildValue("(NNN)", out, kept[0], kept[1]));
+}
+ENTRY(layer_norm) { return norm_forward(M_NORM, self, args, nargs, kwnames); }
+ENTRY(layer_norm_keep) { return norm_forward(M_NORM_KEEP, self, args, nargs, kwnames); }
+
+ENTRY(layer_norm_backward) {
+    static const char *const names[] = {"x", "dy", "mean", "rstd", "weight", "has_bias"};
+    DeviceObject *d = (DeviceObject *)self;
+    PyObject *o[6];
+    View x, dy, mean, rstd, w;
+    int n = 0, has_bias, st;
+    int64_t rows, cols;
+    if (!parse(args, nargs, kwnames, names, 6, 4, o) || !plain(d) || !view_of(o[0], 0, 0, d->index, &x) ||
+        !view_of(o[1], 0, 0, d->index, &dy) || !view_of(o[2], 0, 0, d->index, &mean) ||
+        !view_of(o[3], 0, 0, d->index, &rstd) || !norm_vector(o[4], &x, d->index, &n, &w) || !flag_of(o[5], &has_bias) ||
+        !norm_sizes(&x, n ? n : 1, &rows, &cols) || dy.dtype != x.dtype || dy.ndim != x.ndim ||
+        memcmp(dy.shape, x.shape, (size_t)x.ndim * sizeof(int64_t)) != 0 || mean.dtype != AG_F32 || rstd.dtype != AG_F32 ||
+        count_of(&mean) != rows || count_of(&rstd) != rows)
+        FALL_BACK(M_NORM_BWD);
+    const int64_t *vector = x.shape + (x.ndim - (n ? n : 1));
+    void *dx, *dw = NULL, *db = NULL;
+    PyObject *out = new_tensor(d, x.dtype, x.ndim, x.shape, &dx);
+    PyObject *gw = out == NULL ? NULL : w.p ? new_tensor(d, x.dtype, n, vector, &dw) : Py_NewRef(Py_None);
+    PyObject *gb = gw == NULL ? NULL : has_bias ? new_tensor(d, x.dtype, n ? n : 1, vector, &db) : Py_NewRef(Py_None);
+    if (gb == NULL) {
+        Py_XDECREF(gw);
+        Py_XDECREF(out);
+        return NULL;
+    }
+    CALL(st, p_ag_layer_norm_backward(d->h, (ag_dtype)x.dtype, x.p, w.p, (const float *)mean.p, (const float *)rstd.p, dy.p,
+                                      rows, cols, dx, 0.f, dw, db));
+    return finish(st, Py_BuildValue("(NNN)", out, gw, gb));
+}
+
 /* _bind(handle, stream, index): handle 0 when the device is closed */
 static PyObject *device_bind(PyObject *self, PyObject *args) {
     DeviceObject *d = (DeviceObject *)self;
@@ -541,7 +622,8 @@ static PyObject *device_guarded(PyObject *self, PyObject *on) {
 static PyMethodDef device_methods[] = {
     FAST(dot), FAST(gemm), FAST(dense_forward), FAST(conv2_forward), FAST(conv2_backward_input),
     FAST(conv2_backward_weight), FAST(max_pool2), FAST(max_pool2_backward_from_input), FAST(relu),
-    FAST(relu_backward), FAST(bias_add), FAST(bias_grad),
+    FAST(relu_backward), FAST(bias_add), FAST(bias_grad), FAST(layer_norm), FAST(layer_norm_keep),
+    FAST(layer_norm_backward),
     {"_bind", device_bind, METH_VARARGS, NULL},
     {"_set_guarded", device_guarded, METH_O, NULL},
     {NULL, NULL, 0, NULL}};

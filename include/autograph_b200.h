@@ -385,7 +385,8 @@ AG_API int ag_bias_grad(ag_device *dev, ag_dtype dtype, const void *x, int64_t r
  * The reference has no normalisation layer; these two follow its operators' conventions.  x is
  * viewed as [rows, cols], contiguous; weight and bias [cols] or NULL (ones and zeros).  Sums,
  * statistics and products are f32, each result is rounded once.  A value that is not finite
- * reaches its own row of y or dx and its columns of dweight and dbias, and nothing else. */
+ * reaches its own row of y or dx and its columns of dweight and dbias, and nothing else.
+ * cols < 2^30. */
 
 /* Per row: mean = sum(x) / cols, rstd = 1 / sqrt(sum((x - mean)^2) / cols + eps),
  * y = (x - mean) * rstd * weight + bias.  mean and rstd [rows] (f32) are what the backward pass
