@@ -890,6 +890,8 @@ def _c_specs(spec):
             s.kind, s.c, s.d = _capi.AG_LAYER_MAXPOOL2, layer[1][0], layer[1][1]
         elif kind == "flatten":
             s.kind = _capi.AG_LAYER_FLATTEN
+        elif kind == "layer_norm":   # ("layer_norm", values a row, bias)
+            s.kind, s.a, s.bias = _capi.AG_LAYER_LAYER_NORM, layer[1], int(layer[2])
         else:
             raise ValueError(kind)
     return arr
@@ -959,6 +961,28 @@ class _PyModel:
         _capi.check(lib().ag_model_set_sgd(self._h,
                                            ctypes.c_float(-1.0 if momentum is None else momentum)))
         self.momentum = momentum
+        self.muon = None
+
+    def set_muon(self, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, vector_scale=1.0):
+        """Muon for the weights of Dense and Conv2 layers, SGD with the same momentum and lr * vector_scale for the
+        vectors; clears the momenta.  set_sgd goes back."""
+        _capi.check(lib().ag_model_set_muon(self._h, ctypes.c_float(momentum), int(nesterov), ctypes.c_float(weight_decay),
+                                            steps, ctypes.c_float(vector_scale)))
+        self.momentum = None
+        self.muon = dict(momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=steps,
+                         vector_scale=vector_scale)
+
+    def get_momentum(self, index):
+        """One parameter's momentum in f32, whichever optimizer keeps it."""
+        out = np.empty(self.parameter_lens[index], dtype=np.float32)
+        _capi.check(lib().ag_model_get_momentum(self._h, index, out.ctypes.data))
+        return out
+
+    def set_momenta(self, arrays):
+        for i, a in enumerate(arrays):
+            a = np.ascontiguousarray(a, dtype=np.float32).ravel()
+            assert a.size == self.parameter_lens[i]
+            _capi.check(lib().ag_model_set_momentum(self._h, i, a.ctypes.data))
 
     def get_velocity(self, index):
         return self._fetch(lib().ag_model_get_velocity, index)
@@ -1034,8 +1058,10 @@ class _PyModel:
         params = [self.get_parameter(i) for i in range(n)]
         bf16 = self.dtype == _torch().bfloat16
         # optimizer state travels with the parameters when there is one (SGD with momentum)
-        vel = [self.get_velocity(i) for i in range(n)] if getattr(self, "momentum", None) else None
-        return sf.dumps(sf.model_to_value(self.spec, params, field_names, bf16=bf16, velocities=vel))
+        muon = getattr(self, "muon", None) is not None
+        vel = [self.get_momentum(i) for i in range(n)] if muon or getattr(self, "momentum", None) else None
+        return sf.dumps(sf.model_to_value(self.spec, params, field_names, bf16=bf16, velocities=vel,
+                                          optimizer="Muon" if muon else "SGD"))
 
     def load_serde_json(self, text: str):
         """Loads the parameters of a stack written by to_serde_json or by the reference."""
@@ -1044,8 +1070,11 @@ class _PyModel:
         if [p.size for p in params] != list(self.parameter_lens):
             raise AgError(_capi.AG_ERR_SHAPE, "checkpoint does not match the model's parameters")
         self.set_parameters(params)
-        if all(v is not None for v in states) and getattr(self, "momentum", None):
-            self.set_velocities(states)   # a momentum run continues where it stopped
+        if all(v is not None for v in states):   # a momentum run continues where it stopped
+            if getattr(self, "muon", None) is not None:
+                self.set_momenta(states)
+            elif getattr(self, "momentum", None):
+                self.set_velocities(states)
 
     def forward_device(self, x_dev, out_dev=None):
         bs, c, h, w = x_dev.shape

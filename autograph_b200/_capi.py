@@ -11,6 +11,7 @@ AG_OK = 0
 AG_ERR_INVALID, AG_ERR_SHAPE, AG_ERR_DTYPE, AG_ERR_CUDA = -1, -2, -3, -4
 AG_ERR_OOM, AG_ERR_DEVICE_TIMEOUT, AG_ERR_UNSUPPORTED, AG_ERR_LIMIT = -5, -6, -7, -8
 AG_LAYER_CONV2, AG_LAYER_RELU, AG_LAYER_MAXPOOL2, AG_LAYER_FLATTEN, AG_LAYER_DENSE = 0, 1, 2, 3, 4
+AG_LAYER_LAYER_NORM = 5
 
 _STATUS_NAMES = {
     -1: "AG_ERR_INVALID", -2: "AG_ERR_SHAPE", -3: "AG_ERR_DTYPE", -4: "AG_ERR_CUDA",
@@ -165,6 +166,9 @@ _SIGNATURES = {
     "ag_model_set_sgd": (c_int, [_P, c_float]),
     "ag_model_get_velocity": (c_int, [_P, c_int32, _P]),
     "ag_model_set_velocity": (c_int, [_P, c_int32, _P]),
+    "ag_model_set_muon": (c_int, [_P, c_float, c_int, c_float, c_int32, c_float]),
+    "ag_model_get_momentum": (c_int, [_P, c_int32, _P]),
+    "ag_model_set_momentum": (c_int, [_P, c_int32, _P]),
     "ag_model_set_grad_scale": (c_int, [_P, c_float]),
     "ag_model_infer": (c_int, [_P, _P, c_int64, c_int64, c_int64, c_int64, _P]),
     "ag_model_forward_device": (c_int, [_P, _P, c_int64, c_int64, c_int64, c_int64, _P]),

@@ -475,6 +475,85 @@ class Flatten : public Layer {
     }
 };
 
+// Layer norm over the last `size` values of each row (the trailing dimensions of the input), with a learned weight and, where
+// has_bias, bias per value.  The reference has no normalisation layer; this one follows its layers' conventions.  One kernel
+// computes all three gradients: the first edge asked for its gradient runs it, straight into the parameters' gradient
+// storage where that is still unset.
+class LayerNorm : public Layer {
+   public:
+    Parameter weight;  // [size]
+    bool has_bias = true;
+    Parameter bias;    // [size]
+    static constexpr float eps = 1e-5f;
+
+    const char *name() const override { return "LayerNorm"; }
+    void parameters(std::vector<Parameter *> &out) override {
+        out.push_back(&weight);
+        if (has_bias) out.push_back(&bias);
+    }
+    Variable forward(Pool &pool, const Variable &input) override {
+        const Tensor &x = input.value;
+        const int64_t size = weight.value.len();
+        int64_t cols = 1;
+        size_t d = x.ndim();
+        while (d > 1 && cols < size) cols *= x.dim(--d);
+        if (cols != size)
+            throw Error(AG_ERR_SHAPE, "LayerNorm: the input's trailing dimensions do not hold " + std::to_string(size) +
+                                          " values");
+        if (!x.is_standard_layout()) throw Error(AG_ERR_SHAPE, "LayerNorm needs standard layout");
+        const int64_t rows = x.len() / size;
+        Variable w = weight.to_variable();
+        Variable b = has_bias ? bias.to_variable() : Variable{};
+        const bool recording = input.node || w.node || b.node;
+        Tensor y = !recording && x.exclusive() ? x : Tensor::uninit(pool, x.shape(), x.dtype());
+        Tensor stats = recording ? Tensor::uninit(pool, {2, rows}, AG_F32) : Tensor{};
+        float *mean = recording ? (float *)stats.data() : nullptr;
+        check(ag_layer_norm_forward(x.device(), x.dtype(), x.data(), w.value.data(), has_bias ? b.value.data() : nullptr,
+                                    rows, size, eps, y.data(), mean, recording ? mean + rows : nullptr));
+        if (!recording) return Variable{y, nullptr};
+        struct Grads {
+            bool done = false;
+            Tensor dx, dw, db;
+        };
+        auto st = std::make_shared<Grads>();
+        Pool *pp = &pool;
+        Tensor xv = x, wv = w.value;
+        std::shared_ptr<Node> in_node = input.node, wn = w.node, bn = b.node;
+        auto ensure = [=](const Tensor &dy) {
+            if (st->done) return;
+            auto target = [&](const std::shared_ptr<Node> &n) {
+                if (!n->has_grad && n->grad_storage.defined()) return n->grad_storage;
+                return Tensor::uninit(*pp, {size}, xv.dtype());
+            };
+            if (in_node) st->dx = Tensor::uninit(*pp, xv.shape(), xv.dtype());
+            if (wn) st->dw = target(wn);
+            if (bn) st->db = target(bn);
+            const float *m = (const float *)stats.data();
+            check(ag_layer_norm_backward(xv.device(), xv.dtype(), xv.data(), wv.data(), m, m + rows, dy.data(), rows, size,
+                                         in_node ? st->dx.data() : nullptr, 0.f, wn ? st->dw.data() : nullptr,
+                                         bn ? st->db.data() : nullptr));
+            st->done = true;
+        };
+        VariableBuilder builder;
+        if (in_node)
+            builder.edge(in_node, [=](const Tensor &dy, Tensor *) {
+                ensure(dy);
+                return st->dx;
+            });
+        if (wn)
+            builder.edge(wn, [=](const Tensor &dy, Tensor *) {
+                ensure(dy);
+                return st->dw;
+            });
+        if (bn)
+            builder.edge(bn, [=](const Tensor &dy, Tensor *) {
+                ensure(dy);
+                return st->db;
+            });
+        return builder.build(y);
+    }
+};
+
 // Variable2::cross_entropy_loss (neural_network/criterion.rs:30-77): the value
 // is the summed loss as a host f32; the edge is dx = (dy/bs)(softmax - onehot).
 struct Loss {

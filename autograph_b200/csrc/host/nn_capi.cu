@@ -56,6 +56,7 @@ struct TrainEntry {
     int64_t bs = 0, c = 0, h = 0, w = 0;
     float lr = 0.f, momentum = 0.f, grad_scale = 1.f;
     bool use_momentum = false;
+    uint64_t rule = 0;         // Muon's setting at the capture (ag_model::muon_rule), 0: SGD
     bool with_update = true;   // the optimizer step is part of the graph
     bool from_device = false;  // inputs are device buffers (copied device to device)
     Tensor x_stage, t_stage;
@@ -109,6 +110,16 @@ struct ag_model {
     Tensor values, grads, velocity;  // flat buckets [bucket_len]
     bool use_momentum = false;
     float momentum = 0.f;
+    // Muon for the parameters that are matrices or filter banks, with an f32 momentum bucket of its own; the others keep SGD
+    // with momentum (ag_model_set_muon).
+    struct Muon {
+        bool on = false;
+        float momentum = 0.f, weight_decay = 0.f, vector_scale = 1.f;
+        int nesterov = 0, steps = 0;
+        Tensor velocity;   // f32 [bucket_len]
+    } muon;
+    uint64_t muon_settings = 0;   // how often Muon was set
+    uint64_t muon_rule() const { return muon.on ? muon_settings : 0; }
     float grad_scale = 1.f;
     ag_model(ag_device *d, ag_dtype t) : dev(d), dtype(t), pool(d) {
         const char *e = getenv("AG_GRAPH");
@@ -203,6 +214,13 @@ void fill_uniform(ag_model *m, Tensor &dst, float a, Rng &rng) {
     }
 }
 
+void fill_ones(ag_model *m, Tensor &dst) {
+    const std::vector<float> f((size_t)dst.len(), 1.f);
+    const std::vector<__nv_bfloat16> h((size_t)dst.len(), __float2bfloat16_rn(1.f));
+    check(ag_upload(m->dev, dst.data(), m->dtype == AG_F32 ? (const void *)f.data() : (const void *)h.data(), dst.nbytes()));
+    check(ag_device_wait(m->dev));
+}
+
 int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
 // Whether the model is LeNet5 (autograph_backend.rs:129-146), whose training steps have kernels of
@@ -235,7 +253,8 @@ void build_model(ag_model *m, const ag_layer_spec *specs, int n, uint64_t seed) 
     struct Pending {
         Parameter *p;
         Shape shape;
-        float a;
+        float a;              // drawn from U(-a, a)
+        int constant = -1;    // or all 0 or 1
     };
     std::vector<Pending> pending;
     for (int i = 0; i < n; ++i) {
@@ -285,6 +304,16 @@ void build_model(ag_model *m, const ag_layer_spec *specs, int n, uint64_t seed) 
                 break;
             }
             case AG_LAYER_FLATTEN: m->layers.push_back(std::make_unique<Flatten>()); break;
+            case AG_LAYER_LAYER_NORM: {
+                if (s.a <= 0) throw Error(AG_ERR_INVALID, "LayerNorm: size must be positive");
+                auto l = std::make_unique<LayerNorm>();
+                l->has_bias = s.bias != 0;
+                pending.push_back({&l->weight, {s.a}, 0.f, 1});
+                if (l->has_bias) pending.push_back({&l->bias, {s.a}, 0.f, 0});
+                m->layers.push_back(std::move(l));
+                m->whole_network = false;   // no one-kernel form has it
+                break;
+            }
             default: throw Error(AG_ERR_INVALID, "unknown layer kind");
         }
     }
@@ -305,7 +334,10 @@ void build_model(ag_model *m, const ag_layer_spec *specs, int n, uint64_t seed) 
         p->value = m->values.narrow0(m->offsets[i], len).into_shape(pending[i].shape);
         p->grad = m->grads.narrow0(m->offsets[i], len).into_shape(pending[i].shape);
         p->velocity = m->velocity.narrow0(m->offsets[i], len).into_shape(pending[i].shape);
-        fill_uniform(m, p->value, pending[i].a, rng);
+        if (pending[i].constant < 0)
+            fill_uniform(m, p->value, pending[i].a, rng);
+        else if (pending[i].constant == 1)
+            fill_ones(m, p->value);   // the bucket is zeros
         m->params.push_back(p);
     }
     plan_fused_train(m);
@@ -930,13 +962,37 @@ float forward_backward(ag_model *m, const Tensor &x, const Tensor &t, float *los
     return loss.value;
 }
 
+// Muon over all matrices in one call, SGD with momentum over the vectors.  A step of every matrix moves its outputs by about
+// as much whatever its shape: the factor sqrt(max(1, outputs / inputs)) with Dense weights [inputs, outputs] and filter banks
+// [outputs, inputs * filter].
+void muon_update(ag_model *m, float lr) {
+    std::vector<ag_muon_matrix> list;
+    for (size_t i = 0; i < m->params.size(); ++i) {
+        Parameter *p = m->params[i];
+        const int64_t len = p->value.len();
+        if (p->value.ndim() < 2) {
+            check(ag_sgd_update_momentum(m->dev, m->dtype, p->value.data(), p->grad.data(), p->velocity.data(), len,
+                                         lr * m->muon.vector_scale, m->muon.momentum));
+            continue;
+        }
+        const int64_t rows = p->value.dim(0), cols = len / rows;
+        const double outs = (double)(p->value.ndim() == 2 ? cols : rows), ins = (double)(p->value.ndim() == 2 ? rows : cols);
+        list.push_back({p->value.data(), p->grad.data(), (float *)m->muon.velocity.data() + m->offsets[i], rows, cols,
+                        (float)std::sqrt(std::max(1.0, outs / ins))});
+    }
+    check(ag_muon_update(m->dev, m->dtype, (int32_t)list.size(), list.data(), lr, m->muon.momentum, m->muon.nesterov,
+                         m->muon.weight_decay, m->muon.steps));
+}
+
 // ≙ model.update(lr, &sgd) (layer.rs:656-658 -> SGD::update, optimizer.rs:389-428), over the
 // flat buckets: element-wise identical to updating each parameter.
 void apply_update(ag_model *m, float lr) {
     if (m->grad_scale != 1.f)
         check(ag_scaled_add(m->dev, m->dtype, m->grad_scale - 1.f, m->grads.data(), m->grads.data(),
                             m->bucket_len));
-    if (m->use_momentum)
+    if (m->muon.on)
+        muon_update(m, lr);
+    else if (m->use_momentum)
         check(ag_sgd_update_momentum(m->dev, m->dtype, m->values.data(), m->grads.data(),
                                      m->velocity.data(), m->bucket_len, lr, m->momentum));
     else
@@ -983,8 +1039,8 @@ bool train_step_fused(ag_model *m, const void *x, const uint8_t *t, int64_t bs, 
         x = xt.data();
     }
     ensure_loss_buffers(m);
-    // a gradient scale other than 1 is applied between the gradients and the update
-    const bool in_kernel = with_update && m->grad_scale == 1.f;
+    // a gradient scale other than 1 is applied between the gradients and the update, and Muon is one of its own
+    const bool in_kernel = with_update && m->grad_scale == 1.f && !m->muon.on;
     const ::ag::lenet_train::Sgd sgd = {in_kernel, m->use_momentum, lr, m->momentum};
     check(::ag::lenet_train::step(m->dev, m->dtype, m->train_net, x, t, bs, m->values.data(), m->grads.data(),
                                   m->velocity.data(), sgd, (float *)pinned_device_pointer(m->loss_pinned)));
@@ -1017,7 +1073,7 @@ bool train_step_graph(ag_model *m, const void *x_host, const uint8_t *t_host, in
         if (t.bs == bs && t.c == c && t.h == h && t.w == w && t.lr == lr &&
             t.momentum == m->momentum && t.use_momentum == m->use_momentum &&
             t.grad_scale == m->grad_scale && t.with_update == with_update &&
-            t.from_device == from_device)
+            t.from_device == from_device && t.rule == m->muon_rule())
             e = &t;
     if (!e && with_update) {
         // A learning rate this shape has not been captured with, while another one has: a
@@ -1051,6 +1107,7 @@ bool train_step_graph(ag_model *m, const void *x_host, const uint8_t *t_host, in
         e->bs = bs; e->c = c; e->h = h; e->w = w;
         e->lr = lr; e->momentum = m->momentum; e->use_momentum = m->use_momentum;
         e->grad_scale = m->grad_scale;
+        e->rule = m->muon_rule();
         e->with_update = with_update;
         e->from_device = from_device;
         e->x_stage = Tensor::uninit(m->pool, {bs, c, h, w}, m->dtype);
@@ -1278,6 +1335,8 @@ int ag_model_get_velocity(ag_model *model, int32_t index, void *host) {
     AG_REQUIRE(model && host, AG_ERR_INVALID, "null argument");
     AG_REQUIRE(index >= 0 && index < (int32_t)model->params.size(), AG_ERR_INVALID,
                "parameter index %d out of range", index);
+    AG_REQUIRE(!model->muon.on || model->params[index]->value.ndim() < 2, AG_ERR_UNSUPPORTED,
+               "Muon's momentum is f32: ag_model_get_momentum");
     Tensor &v = model->params[index]->velocity;
     return ag_download(model->dev, host, v.data(), v.nbytes());
 }
@@ -1286,13 +1345,78 @@ int ag_model_set_velocity(ag_model *model, int32_t index, const void *host) {
     AG_REQUIRE(model && host, AG_ERR_INVALID, "null argument");
     AG_REQUIRE(index >= 0 && index < (int32_t)model->params.size(), AG_ERR_INVALID,
                "parameter index %d out of range", index);
+    AG_REQUIRE(!model->muon.on || model->params[index]->value.ndim() < 2, AG_ERR_UNSUPPORTED,
+               "Muon's momentum is f32: ag_model_set_momentum");
     Tensor &v = model->params[index]->velocity;
     AG_TRY(ag_upload(model->dev, v.data(), host, v.nbytes()));
     return ag_device_wait(model->dev);
 }
 
+int ag_model_set_muon(ag_model *model, float momentum, int nesterov, float weight_decay, int32_t steps,
+                      float vector_scale) {
+    AG_REQUIRE(model != nullptr, AG_ERR_INVALID, "model is null");
+    AG_REQUIRE(momentum >= 0.f && momentum <= 3e38f, AG_ERR_INVALID, "muon: momentum must not be negative");
+    AG_REQUIRE(steps >= 1 && steps <= 20, AG_ERR_INVALID, "muon: steps must be in 1..20");
+    AG_REQUIRE(weight_decay == weight_decay && vector_scale == vector_scale, AG_ERR_INVALID, "muon: a scalar is no number");
+    AG_ENTER(model->dev);
+    AG_HOST_GUARD({
+        for (Parameter *p : model->params)
+            if (p->value.ndim() >= 2 && std::min(p->value.dim(0), p->value.len() / p->value.dim(0)) > 16384)
+                throw Error(AG_ERR_LIMIT, "muon: a parameter's shorter side is beyond 16384");
+        if (!model->muon.velocity.defined())
+            model->muon.velocity = Tensor::uninit(model->pool, {model->bucket_len}, AG_F32);
+        check(ag_fill_zero(model->dev, model->muon.velocity.data(), model->muon.velocity.nbytes()));
+        check(ag_fill_zero(model->dev, model->velocity.data(), model->velocity.nbytes()));
+        model->muon.on = true;
+        model->muon.momentum = momentum;
+        model->muon.nesterov = nesterov ? 1 : 0;
+        model->muon.weight_decay = weight_decay;
+        model->muon.steps = steps;
+        model->muon.vector_scale = vector_scale;
+        ++model->muon_settings;
+    })
+}
+
+// One parameter's momentum as f32, whichever optimizer keeps it.
+static int momentum_copy(ag_model *model, int32_t index, float *host, bool set) {
+    AG_REQUIRE(model && host, AG_ERR_INVALID, "null argument");
+    AG_REQUIRE(index >= 0 && index < (int32_t)model->params.size(), AG_ERR_INVALID,
+               "parameter index %d out of range", index);
+    AG_HOST_GUARD({
+        Parameter *p = model->params[index];
+        const size_t n = (size_t)p->value.len();
+        if (model->muon.on && p->value.ndim() >= 2) {
+            float *v = (float *)model->muon.velocity.data() + model->offsets[index];
+            if (set) {
+                check(ag_upload(model->dev, v, host, n * 4));
+                check(ag_device_wait(model->dev));
+            } else {
+                check(ag_download(model->dev, host, v, n * 4));
+            }
+        } else if (model->dtype == AG_F32) {
+            check(set ? ag_model_set_velocity(model, index, host) : ag_model_get_velocity(model, index, host));
+        } else {
+            std::vector<__nv_bfloat16> h(n);
+            if (set) {
+                for (size_t i = 0; i < n; ++i) h[i] = __float2bfloat16_rn(host[i]);
+                check(ag_model_set_velocity(model, index, h.data()));
+            } else {
+                check(ag_model_get_velocity(model, index, h.data()));
+                for (size_t i = 0; i < n; ++i) host[i] = __bfloat162float(h[i]);
+            }
+        }
+    })
+}
+
+int ag_model_get_momentum(ag_model *model, int32_t index, float *host) { return momentum_copy(model, index, host, false); }
+
+int ag_model_set_momentum(ag_model *model, int32_t index, const float *host) {
+    return momentum_copy(model, index, const_cast<float *>(host), true);
+}
+
 int ag_model_set_sgd(ag_model *model, float momentum) {
     AG_REQUIRE(model != nullptr, AG_ERR_INVALID, "model is null");
+    model->muon.on = false;
     model->use_momentum = momentum >= 0.f;
     model->momentum = momentum >= 0.f ? momentum : 0.f;
     return ag_fill_zero(model->dev, model->velocity.data(), model->velocity.nbytes());
@@ -1453,6 +1577,8 @@ int ag_model_last_loss(ag_model *model, float *loss_host) {
 
 int ag_model_allreduce_update(ag_model *model, ag_comm *comm, int rank, float lr) {
     AG_REQUIRE(model != nullptr && comm != nullptr, AG_ERR_INVALID, "null argument");
+    AG_REQUIRE(!model->muon.on, AG_ERR_UNSUPPORTED,
+               "the fused update is SGD's: with Muon, ag_allreduce_sum on the bucket and ag_model_apply_update");
     AG_ENTER(model->dev);
     AG_TRY(::ag::comm_fused_update(comm, rank, model->dtype, model->grads.data(),
                                    model->values.data(), model->velocity.data(), model->bucket_len,

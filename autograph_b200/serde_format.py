@@ -104,9 +104,11 @@ def _tensor(a: np.ndarray, bf16: bool) -> dict:
     return tensor_to_value(data, bf16)
 
 
-def sgd_state_to_value(velocity: np.ndarray, bf16: bool) -> dict:
-    """SGD's per-parameter state as the reference serialises it (momentum in use)."""
-    return {"name": "SGD",
+def sgd_state_to_value(velocity: np.ndarray, bf16: bool, name: str = "SGD") -> dict:
+    """SGD's per-parameter state as the reference serialises it (momentum in use).  Muon's, which the reference does not
+    have, is written the same way under its own name, in f32."""
+    bf16 = bf16 and name == "SGD"
+    return {"name": name,
             "key_values": [["velocity", {"Tensor": {"tensor": _tensor(velocity, bf16),
                                                     "parameter_device": True,
                                                     "parameter_type": True}}]]}
@@ -123,35 +125,37 @@ def sgd_state_from_value(v):
     return None
 
 
-def _param(a: np.ndarray, bf16: bool, velocity=None) -> dict:
+def _param(a: np.ndarray, bf16: bool, velocity=None, optimizer: str = "SGD") -> dict:
     out = {"value": _tensor(a, bf16)}
     if velocity is not None:   # skipped when there is no state (skip_serializing_if)
-        out["optim_state"] = sgd_state_to_value(np.asarray(velocity, np.float32).reshape(a.shape), bf16)
+        out["optim_state"] = sgd_state_to_value(np.asarray(velocity, np.float32).reshape(a.shape), bf16,
+                                                optimizer)
     return out
 
 
-def model_to_value(spec, params, field_names, bf16: bool = False, velocities=None) -> dict:
+def model_to_value(spec, params, field_names, bf16: bool = False, velocities=None, optimizer: str = "SGD") -> dict:
     """A layer stack as the reference would serialise the user's model struct.
 
     spec: the layer list used to build an ``autograph_b200.Model`` (tuples such as
     ("conv", ic, oc, (fh, fw), bias), ("relu",), ("pool", (h, w)), ("flatten",),
     ("dense", inputs, outputs, bias)); params: the parameter arrays in the model's order
     (float32; for a bf16 model the bf16-representable values); field_names: one name per layer;
-    velocities: SGD's velocity per parameter (same order) when momentum is in use, else None.
+    velocities: the momentum per parameter (same order) of SGD with momentum or of Muon (`optimizer`), else None.
     """
     if len(field_names) != len(spec):
         raise ValueError("one field name per layer")
     out, it = {}, iter(params)
     vit = iter(velocities) if velocities is not None else None
     vel = lambda: next(vit) if vit is not None else None
+    param = lambda a: _param(a, bf16, vel(), optimizer)
     for name, layer in zip(field_names, spec):
         kind = layer[0]
         if kind == "conv":
             _, ic, oc, (fh, fw), bias = layer
             w = np.asarray(next(it), np.float32).reshape(oc, ic, fh, fw)
             b = np.asarray(next(it), np.float32).reshape(oc) if bias else None
-            out[name] = {"weight": _param(w, bf16, vel()), "padding": [0, 0], "stride": [1, 1],
-                         "dilation": [1, 1], "bias": _param(b, bf16, vel()) if bias else None}
+            out[name] = {"weight": param(w), "padding": [0, 0], "stride": [1, 1],
+                         "dilation": [1, 1], "bias": param(b) if bias else None}
         elif kind == "dense":
             if len(layer) > 4:
                 raise ValueError("a layer that shares another layer's parameters has no "
@@ -159,8 +163,12 @@ def model_to_value(spec, params, field_names, bf16: bool = False, velocities=Non
             _, ins, outs, bias = layer
             w = np.asarray(next(it), np.float32).reshape(ins, outs)
             b = np.asarray(next(it), np.float32).reshape(outs) if bias else None
-            out[name] = {"weight": _param(w, bf16, vel()),
-                         "bias": _param(b, bf16, vel()) if bias else None}
+            out[name] = {"weight": param(w),
+                         "bias": param(b) if bias else None}
+        elif kind == "layer_norm":   # not a layer of the reference: the layout of its other layers
+            w = np.asarray(next(it), np.float32).reshape(layer[1])
+            b = np.asarray(next(it), np.float32).reshape(layer[1]) if layer[2] else None
+            out[name] = {"weight": param(w), "bias": param(b) if layer[2] else None, "eps": 1e-5}
         elif kind == "pool":
             out[name] = {"filter": [int(layer[1][0]), int(layer[1][1])],
                          "stride": [int(layer[1][0]), int(layer[1][1])]}

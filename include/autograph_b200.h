@@ -499,10 +499,12 @@ typedef enum ag_layer_kind {
     AG_LAYER_RELU = 1,
     AG_LAYER_MAXPOOL2 = 2, /* c = h, d = w (stride = filter, layer.rs:535-539) */
     AG_LAYER_FLATTEN = 3,
-    AG_LAYER_DENSE = 4    /* a = inputs, b = outputs, bias; c = 0, or 1 + the index of an earlier
+    AG_LAYER_DENSE = 4,   /* a = inputs, b = outputs, bias; c = 0, or 1 + the index of an earlier
                            * Dense layer of the same shape whose parameters this layer shares
                            * (one Parameter feeding two layers: its gradients are summed,
                            * autograd.rs:126-131) */
+    AG_LAYER_LAYER_NORM = 5 /* a = values a row (a product of trailing dimensions), bias; eps 1e-5,
+                             * weight ones and bias zeros at the start (ag_layer_norm_forward) */
 } ag_layer_kind;
 
 typedef struct ag_layer_spec {
@@ -536,6 +538,18 @@ AG_API int ag_model_set_sgd(ag_model *model, float momentum);
  * parameter. */
 AG_API int ag_model_get_velocity(ag_model *model, int32_t index, void *host);
 AG_API int ag_model_set_velocity(ag_model *model, int32_t index, const void *host);
+/* Muon (ag_muon_update) for every parameter of two dimensions or more, all in one call, with the
+ * factor sqrt(max(1, outputs / inputs)) on each; vectors (biases, LayerNorm) take SGD with the same
+ * momentum and lr * vector_scale.  Clears the momenta.  ag_model_set_sgd goes back.  A step then
+ * takes the same calls as with SGD, except ag_model_allreduce_update (AG_ERR_UNSUPPORTED: all-reduce
+ * the bucket and call ag_model_apply_update). */
+AG_API int ag_model_set_muon(ag_model *model, float momentum, int nesterov, float weight_decay,
+                             int32_t steps, float vector_scale);
+/* One parameter's momentum in f32 host memory, whichever optimizer keeps it: Muon's is f32 on the
+ * device, and ag_model_get_velocity / _set_velocity refuse it (AG_ERR_UNSUPPORTED); SGD's has the
+ * model's dtype. */
+AG_API int ag_model_get_momentum(ag_model *model, int32_t index, float *host);
+AG_API int ag_model_set_momentum(ag_model *model, int32_t index, const float *host);
 /* Scale applied to gradients before the update (1/world for data parallel). */
 AG_API int ag_model_set_grad_scale(ag_model *model, float scale);
 

@@ -147,6 +147,9 @@ extern "C" {
     pub fn ag_model_set_sgd(model: *mut ag_model, momentum: f32) -> c_int;
     pub fn ag_model_get_velocity(model: *mut ag_model, index: i32, host: *mut c_void) -> c_int;
     pub fn ag_model_set_velocity(model: *mut ag_model, index: i32, host: *const c_void) -> c_int;
+    pub fn ag_model_set_muon(model: *mut ag_model, momentum: f32, nesterov: c_int, weight_decay: f32, steps: i32, vector_scale: f32) -> c_int;
+    pub fn ag_model_get_momentum(model: *mut ag_model, index: i32, host: *mut f32) -> c_int;
+    pub fn ag_model_set_momentum(model: *mut ag_model, index: i32, host: *const f32) -> c_int;
     pub fn ag_model_set_grad_scale(model: *mut ag_model, scale: f32) -> c_int;
     pub fn ag_model_infer(model: *mut ag_model, x_host: *const c_void, bs: i64, c: i64, h: i64, w: i64, logits_host: *mut c_void) -> c_int;
     pub fn ag_model_infer_enqueue(model: *mut ag_model, x_host: *const c_void, bs: i64, c: i64, h: i64, w: i64, logits_host: *mut c_void, ticket: *mut i32) -> c_int;
