@@ -37,23 +37,18 @@ __global__ void __launch_bounds__(256) split_kernel(const __grid_constant__ Grou
     __shared__ double scratch[8];
     __shared__ float tile[64][65];
     int block;
-    const int i = find_matrix(g, block, [](const Matrix &m) { return m.x.plane / 64; });
+    const int i = find_matrix(g, block, [](const Matrix &m) { return m.x(0).plane / 64; });
     const double inv = inverse_norm(g.m[i], parts, scratch);
     split_tile<T>(g.m[i], g.rule, block, inv, planes, tile);
 }
 
-// Rows of the workspace, handed out.
-struct Space {
-    int64_t rows = 0;
-    Stored take(int64_t r, int64_t c) {
-        Stored s;
-        s.rp = (int)(ceil_div(r, 128) * 128);
-        s.plane = (int)(ceil_div(c, 64) * s.rp);
-        s.row = (int)rows;
-        rows += 2 * (int64_t)s.plane;
-        return s;
-    }
-};
+// First step on x x^T alone (muon_product.cuh).  Counted in products of planes of an n x n matrix, for x of r times its size:
+// f32 22.5 r + 7.5 on x throughout, 13.5 r + 16.5 from the third step on; bf16 13.5 r + 4.5 (some steps take one product of
+// planes), 6 r + 20 from the second.  At most five steps: f16 holds no more of q's range.
+static int squares_from(const Matrix &m, int steps, bool bf16) {
+    if (m.n() < 128 || m.wide() < 2 * m.n()) return steps;
+    return std::min(steps, std::max(bf16 ? 1 : 2, steps - 5));
+}
 
 template <class T, int BN>
 static int launch(ag_device *dev, const CUtensorMap &map, __half *planes, double *norms, float4 *slices, const Group &g) {
@@ -83,35 +78,35 @@ int run(ag_device *dev, const std::vector<Matrix> &matrices, const Rule &rule, i
         g.n = (int)std::min<size_t>(kGroup, matrices.size() - first);
         g.steps = steps;
         g.rule = rule;
-        Space space;
+        int64_t space = 0;
         int parts = 0, blocks = 0;
         int64_t values = 0, tiles = 0;
         for (int i = 0; i < g.n; ++i) {
             Matrix &m = g.m[i];
             m = matrices[first + i];
             const int64_t n = std::min(m.rows, m.cols), wide = std::max(m.rows, m.cols);
-            m.x = space.take(n, wide);
-            m.y = space.take(n, wide);
-            m.a = space.take(n, n);
-            m.b = space.take(n, n);
+            m.squares = squares_from(m, steps, sizeof(T) == 2);
+            m.row = (int)std::min<int64_t>(space, INT32_MAX);
+            space += m.space(steps);
+            g.phases = std::max(g.phases, m.phases(steps));
             m.part0 = parts;
             m.parts = (int)std::min<int64_t>(ceil_div(n * wide, 8192), kMostParts);
             parts += m.parts;
-            blocks += m.x.plane / 64;
+            blocks += m.x(0).plane / 64;
             values += n * wide;
             tiles += ceil_div(n, 128) * ceil_div(wide, 128);
         }
-        AG_REQUIRE(space.rows < (1ll << 31), AG_ERR_LIMIT, "newton_schulz: the matrices' workspace is too large");
+        AG_REQUIRE(space < (1ll << 31), AG_ERR_LIMIT, "newton_schulz: the matrices' workspace is too large");
         g.inside = values <= kInside;
         const bool narrow = tiles <= dev->sm_count;
         const size_t heads = (size_t)kGroup * kMostParts * sizeof(double), sums = (size_t)dev->sm_count * 128 * 128 * sizeof(float);
         void *ws;
-        AG_TRY(engine_scratch(dev, heads + sums + (size_t)space.rows * 128, &ws));
+        AG_TRY(engine_scratch(dev, heads + sums + (size_t)space * 128, &ws));
         double *norms = (double *)ws;
         float4 *slices = (float4 *)((char *)ws + heads);
         __half *planes = (__half *)((char *)ws + heads + sums);
         CUtensorMap map;
-        const uint64_t dims[2] = {64, (uint64_t)space.rows}, strides[1] = {64};
+        const uint64_t dims[2] = {64, (uint64_t)space}, strides[1] = {64};
         const uint32_t box[2] = {64, 64};
         AG_TRY(make_tmap_bf16(&map, planes, 2, dims, strides, box));   // f16 has the same size
         if (!g.inside) {
@@ -183,7 +178,7 @@ int ag_newton_schulz(ag_device *dev, ag_dtype dtype, int32_t n, const ag_polar_m
             const uintptr_t bytes = (uintptr_t)(m.rows * m.cols) * dtype_size(dtype);
             ranges.push_back({(uintptr_t)m.g, (uintptr_t)m.g + bytes, false, i, true});
             ranges.push_back({(uintptr_t)m.o, (uintptr_t)m.o + bytes, true, i, true});
-            list.push_back({m.g, m.o, nullptr, m.rows, m.cols, 1.f, 0, 0, {}, {}, {}, {}});
+            list.push_back({m.g, m.o, nullptr, m.rows, m.cols, 1.f, 0, 0, 0, 0});
         }
         AG_TRY(muon::check_overlap(ranges));
         const muon::Rule rule = {0.f, 0.f, 0.f, 0};
@@ -209,7 +204,7 @@ int ag_muon_update(ag_device *dev, ag_dtype dtype, int32_t n, const ag_muon_matr
             ranges.push_back({(uintptr_t)m.g, (uintptr_t)m.g + bytes, false, i, false});
             ranges.push_back({(uintptr_t)m.w, (uintptr_t)m.w + bytes, true, i, false});
             ranges.push_back({(uintptr_t)m.v, (uintptr_t)m.v + count * 4, true, i, false});
-            list.push_back({m.g, m.w, m.v, m.rows, m.cols, m.scale, 0, 0, {}, {}, {}, {}});
+            list.push_back({m.g, m.w, m.v, m.rows, m.cols, m.scale, 0, 0, 0, 0});
         }
         AG_TRY(muon::check_overlap(ranges));
         const muon::Rule rule = {lr, momentum, weight_decay, nesterov ? 1 : 0};

@@ -32,7 +32,25 @@ struct Matrix {
     int64_t rows, cols;
     float scale;
     int part0, parts;   // its partial sums of squares
-    Stored x, y, a, b;
+    int row;            // its first row in the workspace
+    int squares;        // first step that is taken on x x^T alone; the number of steps where none is
+
+    __device__ __host__ __forceinline__ int n() const { return (int)(rows < cols ? rows : cols); }
+    __device__ __host__ __forceinline__ int wide() const { return (int)(rows < cols ? cols : rows); }
+    // x and its successor, n x wide, and the n x n matrices of the steps
+    __device__ __host__ __forceinline__ Stored x(int i) const {
+        const int rp = (n() + 127) / 128 * 128, plane = (wide() + 63) / 64 * rp;
+        return {row + i * 2 * plane, rp, plane};
+    }
+    __device__ __host__ __forceinline__ Stored square(int i) const {
+        const int rp = (n() + 127) / 128 * 128, plane = (n() + 63) / 64 * rp, after = (wide() + 63) / 64 * rp * 4;
+        return {row + after + i * 2 * plane, rp, plane};
+    }
+    __device__ __host__ __forceinline__ int64_t space(int steps) const {   // rows
+        const int64_t rp = (n() + 127) / 128 * 128;
+        return 4 * rp * ((wide() + 63) / 64) + (squares < steps ? 12 : 4) * rp * ((n() + 63) / 64);
+    }
+    __device__ __host__ __forceinline__ int phases(int steps) const { return 3 * steps + (squares < steps); }
 };
 
 // The update's scalars.
@@ -43,7 +61,7 @@ struct Rule {
 
 constexpr int kGroup = 24;   // matrices of a launch: its parameters stay below 4 KB
 struct Group {
-    int n, steps;
+    int n, steps, phases;
     int inside;              // the kernel makes the momenta, norms and planes too
     Rule rule;
     Matrix m[kGroup];
@@ -59,10 +77,12 @@ struct Job {
     int has_e, final;
     int planes;        // of each operand: 2 for hi.hi + hi.lo + lo.hi, 1 for hi.hi
     float c0, c1;
+    float diagonal;    // added to D's
 };
 
 constexpr float kA = 3.4445f, kB = -4.7750f, kC = 2.0315f;
-// Scales of the stored matrices.  |x| <= 1.21, |a| <= 1.46 and |b| <= 2.81 by their norms, f16 ends at 65504.
+// Scales of the stored matrices.  |x| <= 1.21, |a| <= 1.46, |b| <= 2.81, |p| <= 3.45 and |p a| <= 1.2 by their norms, f16
+// ends at 65504; a product of i + 1 factors p is below 3.45^(i + 1) and has the scale kScaleB / 4^i.
 constexpr float kScaleX = 32768.f, kScaleA = 32768.f, kScaleB = 16384.f;
 
 using namespace tc;
@@ -169,6 +189,11 @@ __device__ __forceinline__ void finish32(const Job &j, const Matrix &m, const Ru
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] *= j.c0;
     }
+    if (j.diagonal != 0.f) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+            if (row == col + i && row < j.M) v[i] += j.diagonal;
+    }
     if (j.final) {
 #pragma unroll
         for (int b = 0; b < 32; b += 8) {
@@ -263,8 +288,9 @@ template <class T>
 __device__ __forceinline__ void split_tile(const Matrix &m, const Rule &r, int block, double inv, __half *planes,
                                            float (*tile)[65]) {
     const bool flip = m.rows > m.cols;
-    const int N = (int)(flip ? m.cols : m.rows), M = (int)(flip ? m.rows : m.cols), tiles = m.x.rp / 64;
+    const int N = (int)(flip ? m.cols : m.rows), M = (int)(flip ? m.rows : m.cols), tiles = m.x(0).rp / 64;
     const int i0 = block % tiles * 64, j0 = block / tiles * 64;
+    const Stored xs = m.x(0);
     for (int t = threadIdx.x; t < 64 * 64; t += blockDim.x) {
         const int inner = t % 64, outer = t / 64, i = i0 + (flip ? inner : outer), j = j0 + (flip ? outer : inner);
         float x = 0.f;
@@ -279,9 +305,9 @@ __device__ __forceinline__ void split_tile(const Matrix &m, const Rule &r, int b
         for (int k = 0; k < 8; ++k) v[k] = tile[i][c + k];
         uint4 hi, lo;
         split8(v, hi, lo);
-        const int64_t to = at(m.x, i0 + i, j0 + c);
+        const int64_t to = at(xs, i0 + i, j0 + c);
         *reinterpret_cast<uint4 *>(planes + to) = hi;
-        *reinterpret_cast<uint4 *>(planes + to + (int64_t)m.x.plane * 64) = lo;
+        *reinterpret_cast<uint4 *>(planes + to + (int64_t)xs.plane * 64) = lo;
     }
     __syncthreads();
 }
@@ -303,47 +329,103 @@ __device__ __forceinline__ int planes_of(bool bf16, int n, int step, int steps) 
     return bf16 && n >= 128 && (left == 0 || left > 2) ? 1 : 2;
 }
 
-// Product `phase` (three a step) of a matrix.
+// The products of a matrix, phase by phase.  On x itself a step is
+//   kGram a = x x^T, kPoly b = B a + C a a, kApply x = A x + b x.
+// From step `squares` on the steps need n x n matrices alone: every p = A + B a + C a a is a polynomial of the same a, so that
+// they commute, x stays where it is, and
+//   kFactor p = A + B a + C a a, kHalf r = p a beside kGather q = p q, kNext a = p r, ..., at last kFinish x = q x:
+// four symmetric products a step instead of the long ones.  What the rounding of a leaves of small singular values is relative
+// to the square of the largest, and grows by A^2 a step: a matrix of rank one with 1300 columns was 1.2e-2 off in bf16 with all
+// five steps taken so.  Steps on x itself come first: one for a bf16 result, two for f32.
+enum Kind { kNone = -1, kGram, kPoly, kApply, kFactor, kHalf, kGather, kNext, kFinish };
+struct Phase {
+    int first, second;   // kinds
+    int step;            // of `squares` on: counted from there
+};
+__device__ __forceinline__ Phase phase_of(const Matrix &m, int phase, int steps) {
+    if (phase < 3 * m.squares) return {phase < 3 * steps ? phase % 3 : kNone, kNone, phase / 3};
+    const int q = phase - 3 * m.squares, all = steps - m.squares, i = (q - 1) / 3;
+    if (q == 0) return {all > 0 ? kGram : kNone, kNone, m.squares};
+    if (i >= all) return {kNone, kNone, 0};
+    const bool last = i + 1 == all;
+    switch ((q - 1) % 3) {
+        case 0: return {kFactor, kNone, i};
+        case 1: return last ? Phase{i > 0 ? kGather : kNone, kNone, i} : Phase{kHalf, i > 0 ? kGather : kNone, i};
+        default: return {last ? kFinish : kNext, kNone, i};
+    }
+}
+__device__ __forceinline__ bool is_symmetric(int kind) { return kind != kApply && kind != kFinish; }
+
 template <class T>
-__device__ __forceinline__ Job make_job(const Matrix &m, int phase, int steps) {
-    const int s = phase / 3, n = (int)min(m.rows, m.cols), long_side = (int)max(m.rows, m.cols);
-    const Stored x = s % 2 == 0 ? m.x : m.y, y = s % 2 == 0 ? m.y : m.x;
+__device__ __forceinline__ Job make_job(const Matrix &m, int kind, int step, int steps) {
+    const int n = m.n(), wide = m.wide();
+    const int at_x = kind == kFinish ? m.squares % 2 : step % 2;   // x moves with every step on x itself
+    const Stored x = m.x(at_x), a = m.square(0);
+    // p and the product q of all p so far change places; the first q is the first p
+    const Stored p = m.square(1 + step % 2), q_old = step < 2 ? m.square(1) : m.square(4 + step % 2), q_new = m.square(4 + (step + 1) % 2);
+    const float scale_q = kScaleB * exp2f(-2.f * (float)step), scale_old = kScaleB * exp2f(-2.f * (float)(step - 1));
     Job j;
-    j.planes = planes_of(sizeof(T) == 2, n, s, steps);
+    j.planes = kind <= kApply && step < m.squares ? planes_of(sizeof(T) == 2, n, step, steps) : 2;
     j.final = 0;
     j.M = n;
-    if (phase % 3 == 0) {          // a = x x^T
-        j.p = j.q = j.e = x;
-        j.d = m.a;
-        j.q_mn = 0;
-        j.N = n;
-        j.steps = (long_side + 63) / 64;
-        j.symmetric = 1;
-        j.has_e = 0;
-        j.c0 = kScaleA / (kScaleX * kScaleX);
-        j.c1 = 0.f;
-    } else if (phase % 3 == 1) {   // b = B a + C a a
-        j.p = j.q = j.e = m.a;
-        j.d = m.b;
-        j.q_mn = 0;
-        j.N = n;
-        j.steps = (n + 63) / 64;
-        j.symmetric = 1;
-        j.has_e = 1;
-        j.c0 = kC * kScaleB / (kScaleA * kScaleA);
-        j.c1 = kB * kScaleB / kScaleA;
-    } else {                       // x = A x + b x
-        j.p = m.b;
-        j.q = j.e = x;
-        j.d = y;
-        j.q_mn = 1;
-        j.N = long_side;
-        j.steps = (n + 63) / 64;
-        j.symmetric = 0;
-        j.has_e = 1;
-        j.final = s + 1 == steps;
-        j.c0 = 1.f / (kScaleB * (j.final ? kScaleX : 1.f));
-        j.c1 = j.final ? kA / kScaleX : kA;
+    j.N = n;
+    j.q_mn = 0;
+    j.steps = ((kind == kGram ? wide : n) + 63) / 64;
+    j.symmetric = is_symmetric(kind);
+    j.has_e = 0;
+    j.c1 = 0.f;
+    j.diagonal = 0.f;
+    switch (kind) {
+        case kGram:
+            j.p = j.q = j.e = x;
+            j.d = a;
+            j.c0 = kScaleA / (kScaleX * kScaleX);
+            break;
+        case kPoly:
+        case kFactor:
+            j.p = j.q = j.e = a;
+            j.d = kind == kPoly ? m.square(1) : p;
+            j.has_e = 1;
+            j.c0 = kC * kScaleB / (kScaleA * kScaleA);
+            j.c1 = kB * kScaleB / kScaleA;
+            if (kind == kFactor) j.diagonal = kA * kScaleB;
+            break;
+        case kHalf:
+            j.p = p;
+            j.q = j.e = a;
+            j.d = m.square(3);
+            j.c0 = 1.f / kScaleB;
+            break;
+        case kNext:
+            j.p = p;
+            j.q = j.e = m.square(3);
+            j.d = a;
+            j.c0 = 1.f / kScaleB;
+            break;
+        case kGather:
+            j.p = p;
+            j.q = j.e = q_old;
+            j.d = q_new;
+            j.c0 = scale_q / (kScaleB * scale_old);
+            break;
+        case kFinish:
+            j.p = step == 0 ? p : q_new;
+            j.q = j.e = j.d = x;
+            j.q_mn = 1;
+            j.N = wide;
+            j.final = 1;
+            j.c0 = 1.f / (scale_q * kScaleX);
+            break;
+        default:   // kApply
+            j.p = m.square(1);
+            j.q = j.e = x;
+            j.d = m.x(1 - at_x);
+            j.q_mn = 1;
+            j.N = wide;
+            j.has_e = 1;
+            j.final = step + 1 == steps;
+            j.c0 = 1.f / (kScaleB * (j.final ? kScaleX : 1.f));
+            j.c1 = j.final ? kA / kScaleX : kA;
     }
     return j;
 }
@@ -369,9 +451,13 @@ __device__ __forceinline__ void make_plan(const Group &g, int phase, Plan *plan)
     int tiles = 0, steps = 0;
     if (lane < g.n) {
         const Matrix &m = g.m[lane];
-        const int n = (int)min(m.rows, m.cols);
-        tiles = tiles_of<BN>(n, phase % 3 < 2 ? n : (int)max(m.rows, m.cols), phase % 3 < 2);
-        steps = ((int)(phase % 3 == 0 ? max(m.rows, m.cols) : min(m.rows, m.cols)) + 63) / 64;
+        const Phase ph = phase_of(m, phase, g.steps);
+        const int n = m.n();
+        if (ph.first != kNone) {
+            const bool symmetric = is_symmetric(ph.first);
+            tiles = tiles_of<BN>(n, symmetric ? n : m.wide(), symmetric) * (ph.second != kNone ? 2 : 1);   // both symmetric
+            steps = ((ph.first == kGram ? m.wide() : n) + 63) / 64;
+        }
     }
     int sum = tiles;
 #pragma unroll
@@ -394,7 +480,7 @@ __device__ __forceinline__ void make_plan(const Group &g, int phase, Plan *plan)
 }
 
 struct Item {
-    int matrix, m0, n0, k0, k1;
+    int matrix, kind, step, m0, n0, k0, k1;
     bool mirror;
 };
 
@@ -405,9 +491,19 @@ __device__ __forceinline__ Item find_item(const Group &g, const Plan &plan, int 
     int i = 0;
     while (plan.first[i + 1] <= item) ++i;
     const Matrix &m = g.m[i];
-    const int n = (int)min(m.rows, m.cols), tm = (n + 127) / 128;
+    const Phase ph = phase_of(m, phase, g.steps);
+    const int n = m.n(), tm = (n + 127) / 128;
     int t = item - plan.first[i], bi, bj;
-    if (phase % 3 < 2) {
+    it.kind = ph.first;
+    it.step = ph.step;
+    if (is_symmetric(ph.first)) {
+        if (ph.second != kNone) {
+            const int half = (plan.first[i + 1] - plan.first[i]) / 2;
+            if (t >= half) {
+                t -= half;
+                it.kind = ph.second;
+            }
+        }
         bi = 0;
         for (int left = (n + BN - 1) / BN; t >= left; left -= 128 / BN) {
             t -= left;
@@ -420,7 +516,7 @@ __device__ __forceinline__ Item find_item(const Group &g, const Plan &plan, int 
         bi = t - bj * tm;
         it.mirror = false;
     }
-    const int steps = ((int)(phase % 3 == 0 ? max(m.rows, m.cols) : min(m.rows, m.cols)) + 63) / 64;
+    const int steps = ((it.kind == kGram ? m.wide() : n) + 63) / 64;
     const int per = (steps + plan.splits - 1) / plan.splits;
     it.matrix = i;
     it.m0 = bi * 128;
@@ -516,7 +612,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (; w < before + g.m[i].parts; w += gridDim.x) momentum_part<T>(g.m[i], g.rule, w - before, parts, scratch);
         ok = grid_sync(counters, ++barriers * gridDim.x, status, abort_flag);
         for (int w = blockIdx.x, i = 0, before = 0; ok && i < g.n; ++i) {
-            const int blocks = g.m[i].x.plane / 64;
+            const int blocks = g.m[i].x(0).plane / 64;
             if (w < before + blocks) {
                 const double inv = inverse_norm(g.m[i], parts, scratch);
                 for (; w < before + blocks; w += gridDim.x)
@@ -531,7 +627,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     int stages = 0, accs = 0;
     if (warp == 0) make_plan<BN>(g, 0, plans);
     __syncthreads();
-    for (int phase = 0; ok && phase < 3 * g.steps; ++phase) {
+    for (int phase = 0; ok && phase < g.phases; ++phase) {
         const Plan *plan = plans + phase % 2;
         const int units = plan->items * plan->splits, splits = plan->splits;
         // Where this CTA's first item lies does not depend on what the others still compute.
@@ -539,7 +635,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         Job j = {};
         if ((int)blockIdx.x < units) {
             it = find_item<BN>(g, *plan, blockIdx.x, phase);
-            j = make_job<T>(g.m[it.matrix], phase, g.steps);
+            j = make_job<T>(g.m[it.matrix], it.kind, it.step, g.steps);
         }
         if (phase > 0) {
             ok = grid_sync(counters, ++barriers * gridDim.x, status, abort_flag);
@@ -549,7 +645,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int w = blockIdx.x; w < units; w += gridDim.x) {
                 if (w != (int)blockIdx.x) {
                     it = find_item<BN>(g, *plan, w, phase);
-                    j = make_job<T>(g.m[it.matrix], phase, g.steps);
+                    j = make_job<T>(g.m[it.matrix], it.kind, it.step, g.steps);
                 }
                 const int per = j.planes == 2 ? 1 : 2, count = (it.k1 - it.k0 + per - 1) / per;
                 if (elect_one()) {
@@ -582,7 +678,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int w = blockIdx.x; w < units; w += gridDim.x) {
                 if (w != (int)blockIdx.x) {
                     it = find_item<BN>(g, *plan, w, phase);
-                    j = make_job<T>(g.m[it.matrix], phase, g.steps);
+                    j = make_job<T>(g.m[it.matrix], it.kind, it.step, g.steps);
                 }
                 const int per = j.planes == 2 ? 1 : 2, count = (it.k1 - it.k0 + per - 1) / per;
                 if (elect_one()) {
@@ -636,7 +732,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int w = blockIdx.x; w < units; w += gridDim.x) {
                 if (w != (int)blockIdx.x) {
                     it = find_item<BN>(g, *plan, w, phase);
-                    j = make_job<T>(g.m[it.matrix], phase, g.steps);
+                    j = make_job<T>(g.m[it.matrix], it.kind, it.step, g.steps);
                 }
                 const Matrix &m = g.m[it.matrix];
                 const int col = it.n0 + half * COLS;
@@ -718,7 +814,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 __syncwarp();   // rows beyond the matrix leave the last step's stores early, and what follows takes whole warps
             }
         }
-        if (warp == 0 && phase + 1 < 3 * g.steps) make_plan<BN>(g, phase + 1, plans + (phase + 1) % 2);
+        if (warp == 0 && phase + 1 < g.phases) make_plan<BN>(g, phase + 1, plans + (phase + 1) % 2);
         __syncthreads();
     }
 
