@@ -29,7 +29,7 @@ __global__ void __launch_bounds__(256) momentum_kernel(const __grid_constant__ G
     __shared__ double scratch[8];
     int part;
     const int i = find_matrix(g, part, [](const Matrix &m) { return m.parts; });
-    momentum_part<T>(g.m[i], g.rule, part, parts, scratch);
+    momentum_part<T, 256>(g.m[i], g.rule, part, parts, scratch);
 }
 
 template <class T>
@@ -39,7 +39,7 @@ __global__ void __launch_bounds__(256) split_kernel(const __grid_constant__ Grou
     int block;
     const int i = find_matrix(g, block, [](const Matrix &m) { return m.x(0).plane / 64; });
     const double inv = inverse_norm(g.m[i], parts, scratch);
-    split_tile<T>(g.m[i], g.rule, block, inv, planes, tile);
+    split_tile<T, 256>(g.m[i], g.rule, block, inv, planes, tile);
 }
 
 // First step on x x^T alone (muon_product.cuh).  Counted in products of planes of an n x n matrix, for x of r times its size:

@@ -59,7 +59,7 @@ struct Rule {
     int nesterov;
 };
 
-constexpr int kGroup = 24;   // matrices of a launch: its parameters stay below 4 KB
+constexpr int kGroup = 32;   // matrices of a launch: a lane each, and its parameters stay below 4 KB
 struct Group {
     int n, steps, phases;
     int inside;              // the kernel makes the momenta, norms and planes too
@@ -118,42 +118,52 @@ __device__ __forceinline__ void join8(const uint4 &hi, const uint4 &lo, float (&
     }
 }
 
-// Eight neighbouring values of a row of the result from x: o = x, or w = (1 - lr * decay) * w - lr * scale * x.
-template <class T>
-__device__ __forceinline__ void store_final(const Matrix &m, const Rule &r, int M, int N, int row, int col, const float (&x)[8]) {
+// COLS neighbouring values of a row of the result from x: o = x, or w = (1 - lr * decay) * w - lr * scale * x.  All of w is
+// loaded before any of it is stored.
+template <class T, int COLS>
+__device__ __forceinline__ void store_final(const Matrix &m, const Rule &r, int M, int N, int row, int col, const float *x) {
     if (row >= M || col >= N) return;
     T *o = reinterpret_cast<T *>(m.o);
     const bool update = m.v != nullptr;
     const float keep = 1.f - r.lr * r.decay, step = -r.lr * m.scale;
-    if (m.rows > m.cols) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (col + i < N) {
-                T *p = o + (int64_t)(col + i) * m.cols + row;
-                *p = from_f32<T>(update ? fmaf(step, x[i], keep * to_f32(*p)) : x[i]);
-            }
-        return;
-    }
-    T *p = o + (int64_t)row * m.cols + col;
+    const bool flip = m.rows > m.cols;
     constexpr int V = 16 / (int)sizeof(T);
-    if (col + 8 <= N && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+    T *p = flip ? o + (int64_t)col * m.cols + row : o + (int64_t)row * m.cols + col;
+    if (!flip && col + COLS <= N && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+        uint4 w[COLS / V];
 #pragma unroll
-        for (int b = 0; b < 8; b += V) {
-            union {
-                uint4 raw;
-                T v[V];
-            } w;
-            if (update) w.raw = *reinterpret_cast<const uint4 *>(p + b);
+        for (int b = 0; b < COLS / V; ++b) w[b] = update ? reinterpret_cast<const uint4 *>(p)[b] : make_uint4(0, 0, 0, 0);
 #pragma unroll
-            for (int i = 0; i < V; ++i)
-                w.v[i] = from_f32<T>(update ? fmaf(step, x[b + i], keep * to_f32(w.v[i])) : x[b + i]);
-            *reinterpret_cast<uint4 *>(p + b) = w.raw;
+        for (int b = 0; b < COLS / V; ++b) {
+            uint32_t u[4] = {w[b].x, w[b].y, w[b].z, w[b].w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (V == 4) {
+                    const float v = x[b * V + i];
+                    u[i] = __float_as_uint(update ? fmaf(step, v, keep * __uint_as_float(u[i])) : v);
+                } else {
+                    float lo = x[b * V + 2 * i], hi = x[b * V + 2 * i + 1];
+                    if (update) {
+                        lo = fmaf(step, lo, keep * __uint_as_float(u[i] << 16));
+                        hi = fmaf(step, hi, keep * __uint_as_float(u[i] & 0xffff0000u));
+                    }
+                    const __nv_bfloat162 both = __floats2bfloat162_rn(lo, hi);
+                    u[i] = *reinterpret_cast<const uint32_t *>(&both);
+                }
+            }
+            reinterpret_cast<uint4 *>(p)[b] = make_uint4(u[0], u[1], u[2], u[3]);
         }
         return;
     }
+    const int64_t next = flip ? m.cols : 1;
+    T w[COLS];
+    if (update)
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-        if (col + i < N) p[i] = from_f32<T>(update ? fmaf(step, x[i], keep * to_f32(p[i])) : x[i]);
+        for (int i = 0; i < COLS; ++i)
+            if (col + i < N) w[i] = p[i * next];
+#pragma unroll
+    for (int i = 0; i < COLS; ++i)
+        if (col + i < N) p[i * next] = from_f32<T>(update ? fmaf(step, x[i], keep * to_f32(w[i])) : x[i]);
 }
 
 // Columns col .. col + 31 (col a multiple of 32) of a row of D from their sums, by whole warps whose lanes have neighbouring
@@ -196,12 +206,7 @@ __device__ __forceinline__ void finish32(const Job &j, const Matrix &m, const Ru
     }
     if (j.final) {
 #pragma unroll
-        for (int b = 0; b < 32; b += 8) {
-            float x[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = v[b + i];
-            store_final<T>(m, r, j.M, j.N, row, col + b, x);
-        }
+        for (int b = 0; b < 32; b += 8) store_final<T, 8>(m, r, j.M, j.N, row, col + b, v + b);
         return;
     }
     const int64_t plane = (int64_t)j.d.plane * 64;
@@ -258,18 +263,31 @@ __device__ __forceinline__ double cta_sum(double s, double *scratch) {
 }
 
 // v = momentum * v + g over one part of a matrix, and the part's sum of u^2 in f64 (u^2 itself can exceed f32's range).
-template <class T>
+template <class T, int THREADS>
 __device__ __forceinline__ void momentum_part(const Matrix &m, const Rule &r, int part, double *parts, double *scratch) {
     const int64_t n = m.rows * m.cols, per = (n + m.parts - 1) / m.parts, first = part * per, last = min(n, first + per);
     double s = 0;
-    for (int64_t i = first + threadIdx.x; i < last; i += blockDim.x) {
-        float u = to_f32(reinterpret_cast<const T *>(m.g)[i]);
-        if (m.v != nullptr) {
-            const float v = __fadd_rn(__fmul_rn(r.momentum, m.v[i]), u);
-            m.v[i] = v;
-            u = r.nesterov ? fmaf(r.momentum, v, u) : v;
+    for (int64_t base = first + threadIdx.x; base < last; base += 8 * THREADS) {
+        float u[8], v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int64_t i = base + k * THREADS;
+            u[k] = v[k] = 0.f;
+            if (i < last) {
+                u[k] = to_f32(reinterpret_cast<const T *>(m.g)[i]);
+                if (m.v != nullptr) v[k] = m.v[i];
+            }
         }
-        s += (double)u * (double)u;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int64_t i = base + k * THREADS;
+            if (m.v != nullptr) {
+                v[k] = __fadd_rn(__fmul_rn(r.momentum, v[k]), u[k]);
+                if (i < last) m.v[i] = v[k];
+                u[k] = r.nesterov ? fmaf(r.momentum, v[k], u[k]) : v[k];
+            }
+            s += (double)u[k] * (double)u[k];
+        }
     }
     s = cta_sum(s, scratch);
     if (threadIdx.x == 0) parts[m.part0 + part] = s;
@@ -284,21 +302,22 @@ __device__ __forceinline__ double inverse_norm(const Matrix &m, const double *pa
 }
 
 // 64 x 64 values of x = u / norm(u), transposed where u is taller than wide, as planes.
-template <class T>
+template <class T, int THREADS>
 __device__ __forceinline__ void split_tile(const Matrix &m, const Rule &r, int block, double inv, __half *planes,
                                            float (*tile)[65]) {
     const bool flip = m.rows > m.cols;
     const int N = (int)(flip ? m.cols : m.rows), M = (int)(flip ? m.rows : m.cols), tiles = m.x(0).rp / 64;
     const int i0 = block % tiles * 64, j0 = block / tiles * 64;
     const Stored xs = m.x(0);
-    for (int t = threadIdx.x; t < 64 * 64; t += blockDim.x) {
+#pragma unroll 4
+    for (int t = threadIdx.x; t < 64 * 64; t += THREADS) {
         const int inner = t % 64, outer = t / 64, i = i0 + (flip ? inner : outer), j = j0 + (flip ? outer : inner);
-        float x = 0.f;
-        if (i < N && j < M) x = (float)(direction<T>(m, r, flip ? (int64_t)j * m.cols + i : (int64_t)i * m.cols + j) * inv);
-        tile[i - i0][j - j0] = x;
+        float u = 0.f;
+        if (i < N && j < M) u = direction<T>(m, r, flip ? (int64_t)j * m.cols + i : (int64_t)i * m.cols + j);
+        tile[i - i0][j - j0] = (float)(u * inv);
     }
     __syncthreads();
-    for (int t = threadIdx.x; t < 64 * 8; t += blockDim.x) {
+    for (int t = threadIdx.x; t < 64 * 8; t += THREADS) {
         const int i = t / 8, c = t % 8 * 8;
         float v[8];
 #pragma unroll
@@ -314,11 +333,13 @@ __device__ __forceinline__ void split_tile(const Matrix &m, const Rule &r, int b
 
 // ---- the steps --------------------------------------------------------------------------------------
 
-constexpr int kEpiWarps = 8, kThreads = 64 + kEpiWarps * 32;
+// Warps of a CTA: one issues the loads, one the products, those of the epilogue have 32 rows and half of the columns of the
+// tile each, and one plans the next phase.
+constexpr int kEpilogue = 8, kPlanner = 2 + kEpilogue, kThreads = (kPlanner + 1) * 32;
 constexpr int kBox = 64 * 64 * 2;          // bytes of a box of the tensor map
 // A stage: both planes of 64 k, or the upper one of 128, of 128 rows of P and up to 128 of Q.
 constexpr int kStage = 8 * kBox, kStages = 3;
-constexpr int kSmem = kStages * kStage + 1024 + 512;
+constexpr int kSmem = kStages * kStage + 1024;
 
 // Products of planes of a step.  bf16 results: the products of the last step and of those before the last three are of the
 // planes' upper halves alone.  What an early step rounds off is later drawn to one with the singular values; what the last
@@ -430,99 +451,102 @@ __device__ __forceinline__ Job make_job(const Matrix &m, int kind, int step, int
     return j;
 }
 
-// The work items of a phase: tiles of 128 x BN, of all matrices in a row, each cut in `splits` slices of its depth.
+// The work items of a phase: tiles of 128 rows and BN columns, of all matrices in a row, each cut in `splits` slices of its depth.
 struct Plan {
     int items, splits;
     int first[kGroup + 1];   // of each matrix's tiles
+    int pair[kGroup];        // half of them where there are two products, else none
+    Job job[2][kGroup];
 };
 
 // Tiles of a symmetric product: those that touch the diagonal or lie above it.  With tiles narrower than high, a row of
 // tiles starts at the first that reaches its rows.
-template <int BN>
-__device__ __forceinline__ int tiles_of(int n, int wide, bool symmetric) {
-    const int tm = (n + 127) / 128, tn = (wide + BN - 1) / BN;
-    return symmetric ? tm * tn - 128 / BN * (tm * (tm - 1) / 2) : tm * tn;
+__device__ __forceinline__ int tiles_of(int n, int wide, bool symmetric, int width) {
+    const int tm = (n + 127) / 128, tn = (wide + width - 1) / width;
+    return symmetric ? tm * tn - 128 / width * (tm * (tm - 1) / 2) : tm * tn;
 }
 
-// One warp.
-template <int BN>
+// By one warp.
+template <class T, int BN>
 __device__ __forceinline__ void make_plan(const Group &g, int phase, Plan *plan) {
     const int lane = threadIdx.x % 32;
-    int tiles = 0, steps = 0;
+    int n = 0, wide = 0, copies = 0, steps = 0;
+    bool symmetric = false;
     if (lane < g.n) {
         const Matrix &m = g.m[lane];
         const Phase ph = phase_of(m, phase, g.steps);
-        const int n = m.n();
-        if (ph.first != kNone) {
-            const bool symmetric = is_symmetric(ph.first);
-            tiles = tiles_of<BN>(n, symmetric ? n : m.wide(), symmetric) * (ph.second != kNone ? 2 : 1);   // both symmetric
-            steps = ((ph.first == kGram ? m.wide() : n) + 63) / 64;
-        }
+        n = m.n();
+        symmetric = is_symmetric(ph.first);
+        wide = symmetric ? n : m.wide();
+        copies = ph.first == kNone ? 0 : ph.second == kNone ? 1 : 2;   // a pair is symmetric both
+        if (copies > 0) plan->job[0][lane] = make_job<T>(m, ph.first, ph.step, g.steps);
+        if (copies > 1) plan->job[1][lane] = make_job<T>(m, ph.second, ph.step, g.steps);
+        steps = copies == 0 ? 0 : ((ph.first == kGram ? m.wide() : n) + 63) / 64;
     }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) steps = max(steps, __shfl_xor_sync(0xffffffffu, steps, o));
+    const int tiles = copies * tiles_of(n, wide, symmetric, BN);
     int sum = tiles;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const int up = __shfl_up_sync(0xffffffffu, sum, o);
         if (lane >= o) sum += up;
     }
-    if (lane < g.n) plan->first[lane] = sum - tiles;
-    const int items = __shfl_sync(0xffffffffu, sum, 31);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) steps = max(steps, __shfl_xor_sync(0xffffffffu, steps, o));
-    if (lane == 0) {
-        plan->items = items;
-        plan->first[g.n] = items;
+    if (lane < g.n) {
+        plan->first[lane] = sum - tiles;
+        plan->pair[lane] = copies == 2 ? tiles / 2 : tiles;
+    }
+    if (lane == 31) {
+        plan->items = sum;
+        plan->first[g.n] = sum;
         // Slices while every slice finds an SM at once and has eight steps to take.
-        int splits = 1;
-        while (splits < 8 && 2 * splits * items <= (int)gridDim.x && 16 * splits <= steps) splits *= 2;
-        plan->splits = splits;
+        plan->splits = sum == 0 ? 1 : max(1, min(min((int)gridDim.x / sum, steps / 8), 16));
     }
 }
 
 struct Item {
-    int matrix, kind, step, m0, n0, k0, k1;
+    int matrix, copy, m0, n0, k0, k1;
     bool mirror;
 };
 
 template <int BN>
-__device__ __forceinline__ Item find_item(const Group &g, const Plan &plan, int w, int phase) {
+__device__ __forceinline__ Item find_item(const Plan &plan, int w) {
     Item it;
-    const int item = w / plan.splits, slice = w - item * plan.splits;
+    int item = w, slice = 0;
+    if (plan.splits > 1) {
+        item = w / plan.splits;
+        slice = w - item * plan.splits;
+    }
     int i = 0;
     while (plan.first[i + 1] <= item) ++i;
-    const Matrix &m = g.m[i];
-    const Phase ph = phase_of(m, phase, g.steps);
-    const int n = m.n(), tm = (n + 127) / 128;
     int t = item - plan.first[i], bi, bj;
-    it.kind = ph.first;
-    it.step = ph.step;
-    if (is_symmetric(ph.first)) {
-        if (ph.second != kNone) {
-            const int half = (plan.first[i + 1] - plan.first[i]) / 2;
-            if (t >= half) {
-                t -= half;
-                it.kind = ph.second;
-            }
-        }
+    it.matrix = i;
+    it.copy = t >= plan.pair[i];
+    if (it.copy) t -= plan.pair[i];
+    const Job &j = plan.job[it.copy][i];
+    if (j.symmetric) {
         bi = 0;
-        for (int left = (n + BN - 1) / BN; t >= left; left -= 128 / BN) {
+        for (int left = (j.N + BN - 1) / BN; t >= left; left -= 128 / BN) {
             t -= left;
             ++bi;
         }
         bj = bi * (128 / BN) + t;
         it.mirror = bj * BN >= (bi + 1) * 128;
     } else {
+        const int tm = (j.M + 127) / 128;
         bj = t / tm;
         bi = t - bj * tm;
         it.mirror = false;
     }
-    const int steps = ((it.kind == kGram ? m.wide() : n) + 63) / 64;
-    const int per = (steps + plan.splits - 1) / plan.splits;
-    it.matrix = i;
     it.m0 = bi * 128;
     it.n0 = bj * BN;
-    it.k0 = min(steps, slice * per);
-    it.k1 = min(steps, it.k0 + per);
+    it.k0 = 0;
+    it.k1 = j.steps;
+    if (plan.splits > 1) {
+        const int per = (j.steps + plan.splits - 1) / plan.splits;
+        it.k0 = min(j.steps, slice * per);
+        it.k1 = min(j.steps, it.k0 + per);
+    }
     return it;
 }
 
@@ -559,262 +583,291 @@ __device__ __forceinline__ bool grid_sync(int *arrived, int target, int *status,
     return *abort_flag == 0;
 }
 
+// What the roles of a CTA share.
+struct Cta {
+    const CUtensorMap *map;
+    const Group *g;            // in shared memory
+    __half *planes;
+    float4 *sums;
+    int *counters, *status;
+    uint32_t stages, full, empty, acc_full, acc_empty;   // in shared memory
+    uint32_t tmem;
+    volatile int *abort_flag;
+    int *last_slice;
+    Plan *plans;               // of this phase and of the next, by parity
+};
+
+// Reads a tile's accumulators out, `reads` of them from the accs-th on, adds them and stores the result.
+template <class T, int BN>
+__device__ __forceinline__ void finish_tile(const Cta &t, const Item &it, const Job &j, int w, int splits, int accs, int reads) {
+    constexpr int COLS = BN / 2;
+    const Matrix &m = t.g->m[it.matrix];
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int quarter = warp % 4, part = (warp - 2) / 4, row = quarter * 32 + lane;
+    const int m0 = it.m0, col = it.n0 + part * COLS;
+    Addend e;
+    if (splits == 1) load_addend(j, t.planes, m0 + row, col, e);   // on its way while the products run
+    float sum[COLS];
+#pragma unroll
+    for (int c = 0; c < COLS; ++c) sum[c] = 0.f;
+    bool good = true;
+    for (int c = 0; c < reads; ++c) {
+        const int acc = accs + c;
+        good = __all_sync(0xffffffffu, mbar_wait(t.acc_full + acc % 2 * 8, acc / 2 & 1, t.abort_flag));
+        if (!good) {
+            if (lane == 0) atomicCAS(t.status, 0, 204);
+            break;
+        }
+        tc_fence_after();
+        const uint32_t from = t.tmem + acc % 2 * 128 + part * COLS + ((uint32_t)(quarter * 32) << 16);
+#pragma unroll
+        for (int b = 0; b < COLS; b += 32) {
+            uint32_t v[32];
+            tmem_ld_32x32(from + b, v);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) sum[b + i] += __uint_as_float(v[i]);
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(t.acc_empty + acc % 2 * 8);
+    }
+    __syncwarp();
+    if (splits > 1) {
+        // The slice that is done last adds all of them, in their order, and goes on.  (The warps meet at barriers without a
+        // limit: a CTA has one slice a phase, and all of them come here whether a wait has given up or not.)
+        const int item = w / splits;
+        float4 *mine = t.sums + ((int64_t)w * 32 + part * (COLS / 4)) * 128 + row;
+#pragma unroll
+        for (int c = 0; c < COLS / 4; ++c)
+            __stcg(mine + c * 128, make_float4(sum[4 * c], sum[4 * c + 1], sum[4 * c + 2], sum[4 * c + 3]));
+        __threadfence();
+        asm volatile("bar.sync 1, %0;" ::"n"(kEpilogue * 32) : "memory");
+        if (threadIdx.x == 64) {
+            const int n = atomicAdd(t.counters + 2 + item, 1);
+            if (n == splits - 1) t.counters[2 + item] = 0;
+            *t.last_slice = n == splits - 1;
+            __threadfence();
+        }
+        asm volatile("bar.sync 1, %0;" ::"n"(kEpilogue * 32) : "memory");
+        if (!*t.last_slice) return;
+        load_addend(j, t.planes, m0 + row, col, e);
+#pragma unroll
+        for (int c = 0; c < COLS; ++c) sum[c] = 0.f;
+        for (int z = 0; z < splits; ++z) {
+            const float4 *from = t.sums + (((int64_t)item * splits + z) * 32 + part * (COLS / 4)) * 128 + row;
+#pragma unroll
+            for (int b = 0; b < COLS / 4; b += 8) {
+                float4 p4[8];
+#pragma unroll
+                for (int c = 0; c < 8; ++c) p4[c] = __ldcg(from + (b + c) * 128);
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    sum[4 * (b + c)] += p4[c].x;
+                    sum[4 * (b + c) + 1] += p4[c].y;
+                    sum[4 * (b + c) + 2] += p4[c].z;
+                    sum[4 * (b + c) + 3] += p4[c].w;
+                }
+            }
+        }
+    }
+    if (!good) return;
+#pragma unroll
+    for (int b = 0; b < COLS; b += 32) {
+        if (b > 0) load_addend(j, t.planes, m0 + row, col + b, e);
+        finish32<T>(j, m, t.g->rule, t.planes, m0 + row, col + b, sum + b, e, it.mirror);
+        __syncwarp();   // rows beyond the matrix leave the last step's stores early, and what follows takes whole warps
+    }
+}
+
+// One phase.  stages, accs: stages and accumulators taken so far, which give the place in the rings and
+// the parity of their barriers.  barrier: the arrivals that open it, 0 for the first phase.
+template <class T, int BN>
+__device__ __forceinline__ bool run_phase(const Cta &t, int phase, int barrier, int &stages_taken, int &accs_taken) {
+    // 64-k steps that one accumulator adds: tcgen05 cuts its sums off rather than rounding them, by up to 2^-23 of the sum
+    // so far an addition
+    constexpr int kAccStages = sizeof(T) == 2 ? 16 : 1;
+    constexpr int HALF = (2 + BN / 64) * kBox;   // of a stage: 128 rows of P, BN of Q
+    const Group &g = *t.g;
+    const Plan *plan = t.plans + phase % 2;
+    const int warp = threadIdx.x / 32;
+    const int units = plan->items * plan->splits, splits = plan->splits;
+    int stages = stages_taken, accs = accs_taken;
+    // Where this CTA's first item lies does not depend on what the others still compute.
+    Item first = {};
+    if ((int)blockIdx.x < units) first = find_item<BN>(*plan, blockIdx.x);
+    if (barrier > 0 && !grid_sync(t.counters, barrier, t.status, t.abort_flag)) return false;
+
+    if (warp == kPlanner) {
+        // What does not depend on what the others compute is ready before the next barrier.
+        if (phase + 1 < g.phases) make_plan<T, BN>(g, phase + 1, t.plans + (phase + 1) % 2);
+    } else if (warp == 0) {
+        for (int w = blockIdx.x; w < units; w += gridDim.x) {
+            const Item it = w == (int)blockIdx.x ? first : find_item<BN>(*plan, w);
+            const Job &j = plan->job[it.copy][it.matrix];
+            const bool two = j.planes == 2, q_mn = j.q_mn;
+            const int per = two ? 1 : 2, count = (it.k1 - it.k0 + per - 1) / per;
+            // rows of a step's boxes, and from one to the next
+            const int p_base = j.p.row + it.m0, p_plane = j.p.plane, p_step = j.p.rp;
+            const int q_base = j.q.row + (q_mn ? it.n0 / 64 * j.q.rp : it.n0), q_plane = j.q.plane, q_step = q_mn ? 64 : j.q.rp;
+            const int q_box = q_mn ? j.q.rp : 64;
+            if (elect_one()) {
+                for (int c = 0; c < count; ++c) {
+                    const int at_stage = (stages + c) % kStages, round = (stages + c) / kStages;
+                    if (!mbar_wait(t.empty + at_stage * 8, (round & 1) ^ 1, t.abort_flag)) {
+                        atomicCAS(t.status, 0, 201);
+                        break;
+                    }
+                    const uint32_t bar = t.full + at_stage * 8, dst = t.stages + at_stage * kStage;
+                    const int k = it.k0 + c * per, halves = two || k + 1 < it.k1 ? 2 : 1;
+                    mbar_arrive_expect_tx(bar, halves * HALF);
+                    for (int h = 0; h < halves; ++h) {
+                        const int kk = two ? k : k + h, p_row = p_base + (two ? h * p_plane : 0) + kk * p_step;
+                        const int q_row = q_base + (two ? h * q_plane : 0) + kk * q_step;
+                        const uint32_t to = dst + h * HALF;
+                        tma_load_2d(to, t.map, bar, 0, p_row);
+                        tma_load_2d(to + kBox, t.map, bar, 0, p_row + 64);
+#pragma unroll
+                        for (int b = 0; b < BN / 64; ++b) tma_load_2d(to + (2 + b) * kBox, t.map, bar, 0, q_row + b * q_box);
+                    }
+                }
+            }
+            __syncwarp();
+            stages += count;
+        }
+    } else if (warp == 1) {
+        for (int w = blockIdx.x; w < units; w += gridDim.x) {
+            const Item it = w == (int)blockIdx.x ? first : find_item<BN>(*plan, w);
+            const Job &j = plan->job[it.copy][it.matrix];
+            const bool two = j.planes == 2, q_mn = j.q_mn;
+            const int per = two ? 1 : 2, count = (it.k1 - it.k0 + per - 1) / per;
+            if (elect_one()) {
+                const uint32_t idesc = half_idesc(q_mn, 128, BN);
+                const uint32_t q_step = q_mn ? 16 * 128 : 32, q_lbo = q_mn ? kBox : 0;
+                for (int c = 0; c < count; ++c) {
+                    const int acc = accs + c / kAccStages;
+                    if (c % kAccStages == 0 && !mbar_wait(t.acc_empty + acc % 2 * 8, (acc / 2 & 1) ^ 1, t.abort_flag)) {
+                        atomicCAS(t.status, 0, 202);
+                        break;
+                    }
+                    const int at_stage = (stages + c) % kStages;
+                    if (!mbar_wait(t.full + at_stage * 8, (stages + c) / kStages & 1, t.abort_flag)) {
+                        atomicCAS(t.status, 0, 203);
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t d = t.tmem + acc % 2 * 128, base = t.stages + at_stage * kStage;
+                    auto mma = [&](int hp, int hq, int i, bool add) {
+                        umma_bf16(d, make_smem_desc(base + hp * HALF + i * 32, 0, 1024),
+                                  make_smem_desc(base + hq * HALF + 2 * kBox + i * q_step, q_lbo, 1024), idesc, add ? 1u : 0u);
+                    };
+                    const bool more = c % kAccStages != 0;
+                    if (two) {
+                        // the small products first: what an addition cuts off is a part of the sum so far
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            mma(0, 1, i, more || i > 0);
+                            mma(1, 0, i, true);
+                        }
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) mma(0, 0, i, true);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) mma(0, 0, i, more || i > 0);
+                        if (it.k0 + 2 * c + 1 < it.k1)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) mma(1, 1, i, true);
+                    }
+                    umma_commit(t.empty + at_stage * 8);
+                    if ((c + 1) % kAccStages == 0 || c + 1 == count) umma_commit(t.acc_full + acc % 2 * 8);
+                }
+            }
+            __syncwarp();
+            stages += count;
+            accs += (count + kAccStages - 1) / kAccStages;
+        }
+    } else {
+        for (int w = blockIdx.x; w < units; w += gridDim.x) {
+            const Item it = w == (int)blockIdx.x ? first : find_item<BN>(*plan, w);
+            const Job &j = plan->job[it.copy][it.matrix];
+            const int per = j.planes == 2 ? 1 : 2, count = (it.k1 - it.k0 + per - 1) / per;
+            const int reads = (count + kAccStages - 1) / kAccStages;
+            finish_tile<T, BN>(t, it, j, w, splits, accs, reads);
+            accs += reads;
+        }
+    }
+    stages_taken = stages;
+    accs_taken = accs;
+    return true;
+}
+
 // counters: [0] arrivals at the grid's barrier, [1] CTAs that have left, [2 ...] slices of a tile that are done; zero before
 // and after.  sums: a tile's slices, [item][slice][four columns][row].
 template <class T, int BN>
 __global__ void __launch_bounds__(kThreads, 1)
     muon_kernel(const __grid_constant__ CUtensorMap map, __half *planes, double *parts, float4 *sums, int *counters, int *status,
-                const __grid_constant__ Group g) {
-    constexpr bool BF16 = sizeof(T) == 2;
-    constexpr int COLS = BN / 2, QBOXES = BN / 64;   // of an epilogue warp; of a stage's half
-    constexpr int HALF = (2 + QBOXES) * kBox;
-    // 64-k steps that one accumulator adds: tcgen05 cuts its sums off rather than rounding them, by up to 2^-23 of the sum
-    // so far an addition
-    constexpr int kAccStages = BF16 ? 16 : 1;
+                const __grid_constant__ Group group) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + kStages * kStage);
-    uint64_t *full = bars, *empty = bars + kStages, *acc_full = bars + 2 * kStages, *acc_empty = acc_full + 2;
-    uint32_t *slot = reinterpret_cast<uint32_t *>(acc_empty + 2);
-    volatile int *abort_flag = reinterpret_cast<volatile int *>(slot + 1);
-    int *last_slice = reinterpret_cast<int *>(slot + 2);
-    Plan *plans = reinterpret_cast<Plan *>(slot + 4);
-    double *scratch = reinterpret_cast<double *>(bars + 48);
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    __shared__ uint64_t bars[2 * kStages + 4];
+    __shared__ uint32_t slot;
+    __shared__ int flags[2];
+    __shared__ Plan plans[2];
+    __shared__ Group g;
+    __shared__ double scratch[kThreads / 32];
+    volatile int *abort_flag = flags;
+    const int warp = threadIdx.x / 32;
+    const uint32_t bar0 = smem_u32(bars);
 
     if (threadIdx.x == 0) {
         prefetch_tmap(&map);
         for (int s = 0; s < kStages; ++s) {
-            mbar_init(smem_u32(&full[s]), 1);
-            mbar_init(smem_u32(&empty[s]), 1);
+            mbar_init(bar0 + s * 8, 1);
+            mbar_init(bar0 + (kStages + s) * 8, 1);
         }
         for (int s = 0; s < 2; ++s) {
-            mbar_init(smem_u32(&acc_full[s]), 1);
-            mbar_init(smem_u32(&acc_empty[s]), kEpiWarps);
+            mbar_init(bar0 + (2 * kStages + s) * 8, 1);
+            mbar_init(bar0 + (2 * kStages + 2 + s) * 8, kEpilogue);
         }
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
+    for (int i = threadIdx.x; i < (int)(sizeof(Group) / 4); i += kThreads)
+        reinterpret_cast<uint32_t *>(&g)[i] = reinterpret_cast<const uint32_t *>(&group)[i];
     if (warp == 1) {
-        tmem_alloc(smem_u32(slot), 256);
+        tmem_alloc(smem_u32(&slot), 256);
         tmem_relinquish();
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *slot;
+    const Cta c = {&map, &g, planes, sums, counters, status, smem_u32(smem), bar0, bar0 + kStages * 8, bar0 + 2 * kStages * 8,
+                   bar0 + (2 * kStages + 2) * 8, slot, abort_flag, flags + 1, plans};
     int barriers = 0;
     bool ok = true;
 
     if (g.inside) {
         for (int w = blockIdx.x, i = 0, before = 0; i < g.n; before += g.m[i].parts, ++i)
-            for (; w < before + g.m[i].parts; w += gridDim.x) momentum_part<T>(g.m[i], g.rule, w - before, parts, scratch);
+            for (; w < before + g.m[i].parts; w += gridDim.x) momentum_part<T, kThreads>(g.m[i], g.rule, w - before, parts, scratch);
         ok = grid_sync(counters, ++barriers * gridDim.x, status, abort_flag);
         for (int w = blockIdx.x, i = 0, before = 0; ok && i < g.n; ++i) {
             const int blocks = g.m[i].x(0).plane / 64;
             if (w < before + blocks) {
                 const double inv = inverse_norm(g.m[i], parts, scratch);
                 for (; w < before + blocks; w += gridDim.x)
-                    split_tile<T>(g.m[i], g.rule, w - before, inv, planes, reinterpret_cast<float(*)[65]>(smem));
+                    split_tile<T, kThreads>(g.m[i], g.rule, w - before, inv, planes, reinterpret_cast<float(*)[65]>(smem));
             }
             before += blocks;
         }
-        ok = ok && grid_sync(counters, ++barriers * gridDim.x, status, abort_flag);
     }
 
-    // Stages taken so far, and accumulators: the place in the rings and the parity of their barriers.
     int stages = 0, accs = 0;
-    if (warp == 0) make_plan<BN>(g, 0, plans);
+    if (warp == kPlanner) make_plan<T, BN>(g, 0, plans);
     __syncthreads();
     for (int phase = 0; ok && phase < g.phases; ++phase) {
-        const Plan *plan = plans + phase % 2;
-        const int units = plan->items * plan->splits, splits = plan->splits;
-        // Where this CTA's first item lies does not depend on what the others still compute.
-        Item it = {};
-        Job j = {};
-        if ((int)blockIdx.x < units) {
-            it = find_item<BN>(g, *plan, blockIdx.x, phase);
-            j = make_job<T>(g.m[it.matrix], it.kind, it.step, g.steps);
-        }
-        if (phase > 0) {
-            ok = grid_sync(counters, ++barriers * gridDim.x, status, abort_flag);
-            if (!ok) break;
-        }
-        if (warp == 0) {
-            for (int w = blockIdx.x; w < units; w += gridDim.x) {
-                if (w != (int)blockIdx.x) {
-                    it = find_item<BN>(g, *plan, w, phase);
-                    j = make_job<T>(g.m[it.matrix], it.kind, it.step, g.steps);
-                }
-                const int per = j.planes == 2 ? 1 : 2, count = (it.k1 - it.k0 + per - 1) / per;
-                if (elect_one()) {
-                    for (int c = 0; c < count; ++c) {
-                        const int at_stage = (stages + c) % kStages, round = (stages + c) / kStages;
-                        if (!mbar_wait(smem_u32(&empty[at_stage]), (round & 1) ^ 1, abort_flag)) {
-                            atomicCAS(status, 0, 201);
-                            break;
-                        }
-                        const uint32_t bar = smem_u32(&full[at_stage]), dst = smem_u32(smem + at_stage * kStage);
-                        const int k = it.k0 + c * per, halves = j.planes == 2 || k + 1 < it.k1 ? 2 : 1;
-                        mbar_arrive_expect_tx(bar, halves * HALF);
-                        for (int h = 0; h < halves; ++h) {
-                            const int pl = j.planes == 2 ? h : 0, kk = j.planes == 2 ? k : k + h;
-                            const int p_row = j.p.row + pl * j.p.plane + kk * j.p.rp + it.m0;
-                            const int q_row = j.q.row + pl * j.q.plane + (j.q_mn ? it.n0 / 64 * j.q.rp + kk * 64 : kk * j.q.rp + it.n0);
-                            const uint32_t to = dst + h * HALF;
-                            tma_load_2d(to, &map, bar, 0, p_row);
-                            tma_load_2d(to + kBox, &map, bar, 0, p_row + 64);
-#pragma unroll
-                            for (int b = 0; b < QBOXES; ++b)
-                                tma_load_2d(to + (2 + b) * kBox, &map, bar, 0, q_row + b * (j.q_mn ? j.q.rp : 64));
-                        }
-                    }
-                }
-                __syncwarp();
-                stages += count;
-            }
-        } else if (warp == 1) {
-            for (int w = blockIdx.x; w < units; w += gridDim.x) {
-                if (w != (int)blockIdx.x) {
-                    it = find_item<BN>(g, *plan, w, phase);
-                    j = make_job<T>(g.m[it.matrix], it.kind, it.step, g.steps);
-                }
-                const int per = j.planes == 2 ? 1 : 2, count = (it.k1 - it.k0 + per - 1) / per;
-                if (elect_one()) {
-                    const uint32_t idesc = half_idesc(j.q_mn, 128, BN);
-                    const uint32_t q_step = j.q_mn ? 16 * 128 : 32, q_lbo = j.q_mn ? kBox : 0;
-                    for (int c = 0; c < count; ++c) {
-                        const int acc = accs + c / kAccStages;
-                        if (c % kAccStages == 0 && !mbar_wait(smem_u32(&acc_empty[acc % 2]), (acc / 2 & 1) ^ 1, abort_flag)) {
-                            atomicCAS(status, 0, 202);
-                            break;
-                        }
-                        const int at_stage = (stages + c) % kStages;
-                        if (!mbar_wait(smem_u32(&full[at_stage]), (stages + c) / kStages & 1, abort_flag)) {
-                            atomicCAS(status, 0, 203);
-                            break;
-                        }
-                        tc_fence_after();
-                        const uint32_t d = tmem + acc % 2 * 128, base = smem_u32(smem + at_stage * kStage);
-                        auto mma = [&](int hp, int hq, int i, bool add) {
-                            umma_bf16(d, make_smem_desc(base + hp * HALF + i * 32, 0, 1024),
-                                      make_smem_desc(base + hq * HALF + 2 * kBox + i * q_step, q_lbo, 1024), idesc,
-                                      add ? 1u : 0u);
-                        };
-                        const bool more = c % kAccStages != 0;
-                        if (j.planes == 2) {
-                            // the small products first: what an addition cuts off is a part of the sum so far
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                mma(0, 1, i, more || i > 0);
-                                mma(1, 0, i, true);
-                            }
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) mma(0, 0, i, true);
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) mma(0, 0, i, more || i > 0);
-                            if (it.k0 + 2 * c + 1 < it.k1)
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) mma(1, 1, i, true);
-                        }
-                        umma_commit(smem_u32(&empty[at_stage]));
-                        if ((c + 1) % kAccStages == 0 || c + 1 == count) umma_commit(smem_u32(&acc_full[acc % 2]));
-                    }
-                }
-                __syncwarp();
-                stages += count;
-                accs += (count + kAccStages - 1) / kAccStages;
-            }
-        } else {
-            const int quarter = warp % 4, half = (warp - 2) / 4, row = quarter * 32 + lane;   // of the tile
-            for (int w = blockIdx.x; w < units; w += gridDim.x) {
-                if (w != (int)blockIdx.x) {
-                    it = find_item<BN>(g, *plan, w, phase);
-                    j = make_job<T>(g.m[it.matrix], it.kind, it.step, g.steps);
-                }
-                const Matrix &m = g.m[it.matrix];
-                const int col = it.n0 + half * COLS;
-                Addend e;
-                if (splits == 1) load_addend(j, planes, it.m0 + row, col, e);
-                const int per = j.planes == 2 ? 1 : 2, count = (it.k1 - it.k0 + per - 1) / per;
-                float sum[COLS];
-#pragma unroll
-                for (int c = 0; c < COLS; ++c) sum[c] = 0.f;
-                const int reads = (count + kAccStages - 1) / kAccStages;
-                for (int c = 0; c < reads; ++c) {
-                    const int acc = accs + c;
-                    if (!mbar_wait(smem_u32(&acc_full[acc % 2]), acc / 2 & 1, abort_flag)) {
-                        if (lane == 0) atomicCAS(status, 0, 204);
-                        break;
-                    }
-                    __syncwarp();
-                    tc_fence_after();
-                    const uint32_t t = tmem + acc % 2 * 128 + half * COLS + ((uint32_t)(quarter * 32) << 16);
-#pragma unroll
-                    for (int b = 0; b < COLS; b += 32) {
-                        uint32_t v[32];
-                        tmem_ld_32x32(t + b, v);
-                        tmem_ld_wait();
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) sum[b + i] += __uint_as_float(v[i]);
-                    }
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(smem_u32(&acc_empty[acc % 2]));
-                }
-                accs += reads;
-                __syncwarp();
-                if (*abort_flag) break;
-                if (splits > 1) {
-                    // The slice that is done last adds all of them, in their order, and goes on.
-                    const int item = w / splits;
-                    float4 *mine = sums + ((int64_t)w * 32 + half * (COLS / 4)) * 128 + row;
-#pragma unroll
-                    for (int c = 0; c < COLS / 4; ++c)
-                        __stcg(mine + c * 128, make_float4(sum[4 * c], sum[4 * c + 1], sum[4 * c + 2], sum[4 * c + 3]));
-                    __threadfence();
-                    asm volatile("bar.sync 1, %0;" ::"n"(kEpiWarps * 32) : "memory");
-                    if (threadIdx.x == 64) {
-                        const int n = atomicAdd(counters + 2 + item, 1);
-                        if (n == splits - 1) counters[2 + item] = 0;
-                        *last_slice = n == splits - 1;
-                        __threadfence();
-                    }
-                    asm volatile("bar.sync 1, %0;" ::"n"(kEpiWarps * 32) : "memory");
-                    const bool mine_last = *last_slice;
-                    asm volatile("bar.sync 1, %0;" ::"n"(kEpiWarps * 32) : "memory");
-                    if (!mine_last) continue;
-                    load_addend(j, planes, it.m0 + row, col, e);
-#pragma unroll
-                    for (int c = 0; c < COLS; ++c) sum[c] = 0.f;
-                    for (int z = 0; z < splits; ++z) {
-                        const float4 *from = sums + (((int64_t)item * splits + z) * 32 + half * (COLS / 4)) * 128 + row;
-#pragma unroll
-                        for (int b = 0; b < COLS / 4; b += 8) {
-                            float4 part[8];
-#pragma unroll
-                            for (int c = 0; c < 8; ++c) part[c] = __ldcg(from + (b + c) * 128);
-#pragma unroll
-                            for (int c = 0; c < 8; ++c) {
-                                sum[4 * (b + c)] += part[c].x;
-                                sum[4 * (b + c) + 1] += part[c].y;
-                                sum[4 * (b + c) + 2] += part[c].z;
-                                sum[4 * (b + c) + 3] += part[c].w;
-                            }
-                        }
-                    }
-                }
-#pragma unroll
-                for (int b = 0; b < COLS / 32; ++b) {
-                    if (b > 0) load_addend(j, planes, it.m0 + row, col + b * 32, e);
-                    finish32<T>(j, m, g.rule, planes, it.m0 + row, col + b * 32, sum + b * 32, e, it.mirror);
-                }
-                __syncwarp();   // rows beyond the matrix leave the last step's stores early, and what follows takes whole warps
-            }
-        }
-        if (warp == 0 && phase + 1 < g.phases) make_plan<BN>(g, phase + 1, plans + (phase + 1) % 2);
+        if (phase > 0 || g.inside) ++barriers;
+        ok = run_phase<T, BN>(c, phase, barriers * (int)gridDim.x, stages, accs);
         __syncthreads();
     }
 
@@ -826,7 +879,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (warp == 1) {
         tc_fence_after();
-        tmem_dealloc(tmem, 256);
+        tmem_dealloc(c.tmem, 256);
     }
     // The last CTA to leave, when all have passed the last barrier, clears the counts for the next launch.
     if (threadIdx.x == 0) {
