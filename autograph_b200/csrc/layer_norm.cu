@@ -8,12 +8,14 @@
 // Everything is computed in f32 and rounded once where it is stored; mean and rstd are f32 tensors.
 //
 // Both directions are bound by memory: forward reads x and writes y, backward reads x and dy and writes dx, once each.  A row
-// is held in registers by a group of G threads (a warp, or a whole CTA), up to 32 values a thread, so that its statistics, and
+// is held in registers by a group of G threads (a warp, or a whole CTA), up to 64 values a thread, so that its statistics, and
 // the differences from its mean that the variance is a sum of, cost no second read.  Rows that start on 16 bytes and are
 // whole vectors move 16 bytes a load, others one value, neighbouring lanes on neighbouring values either way.
 // A backward group takes every `groups`-th row and adds dy * hat and dy of its columns in registers as it goes; the CTAs'
 // sums are added in the order of the CTAs, by the CTA that finishes last or, where there is more to add, by a second
 // kernel.  Longer rows take two kernels that read them again.
+// Of the measured copy bandwidth, 65536 x 1024: f32 forward 0.97 (85 us), backward 0.70 (177), bf16 0.86 (48) and 0.72 (86);
+// backward is near its instructions there, about twenty a value; 256 x 25088 f32 forward 0.65 (12 us, half a row an SM at a time).
 //
 // Products that feed a sum are written as __fmul_rn or fmaf: left to the compiler, it fuses them one way in the loop for calls
 // that ask for the statistics, or for one gradient, and another way in the next, and the same values would give other bits.
@@ -339,10 +341,12 @@ __global__ void __launch_bounds__(256) columns_kernel(int parts, int cols, const
     }
 }
 
-template <class T>
+// Rows that no registers hold, VEC values at a time.
+template <class T, int VEC>
 __global__ void __launch_bounds__(1024)
     layer_norm_long_backward_kernel(const T *x, const T *weight, const float *mean, const float *rstd, const T *dy, int64_t rows,
                                     int64_t cols, T *dx) {
+    using P = Pack<T, VEC>;
     __shared__ float scratch[64];
     let_dependents_launch();
     dependency_wait();
@@ -350,44 +354,68 @@ __global__ void __launch_bounds__(1024)
         const T *xr = x + row * cols, *dr = dy + row * cols;
         const float m = mean[row], r = rstd[row];
         float s[2] = {0.f, 0.f};
-#pragma unroll 4
-        for (int64_t i = threadIdx.x; i < cols; i += 1024) {
-            const float hat = __fmul_rn(to_f32(xr[i]) - m, r);
-            float d = to_f32(dr[i]);
-            if (weight != nullptr) d = __fmul_rn(d, to_f32(weight[i]));
-            s[0] += d;
-            s[1] = fmaf(d, hat, s[1]);
+#pragma unroll 2
+        for (int64_t i = threadIdx.x * VEC; i < cols; i += 1024 * VEC) {
+            const P px = *reinterpret_cast<const P *>(xr + i), pd = *reinterpret_cast<const P *>(dr + i);
+            P w;
+            if (weight != nullptr) w = *reinterpret_cast<const P *>(weight + i);
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) {
+                float d = pd.get(k);
+                if (weight != nullptr) d = __fmul_rn(d, w.get(k));
+                s[0] += d;
+                s[1] = fmaf(d, __fmul_rn(px.get(k) - m, r), s[1]);
+            }
         }
         group_sum<1024>(s, scratch);
         const float along = s[0] / (float)cols, across = s[1] / (float)cols;
-#pragma unroll 4
-        for (int64_t i = threadIdx.x; i < cols; i += 1024) {
-            const float hat = __fmul_rn(to_f32(xr[i]) - m, r);
-            float d = to_f32(dr[i]);
-            if (weight != nullptr) d = __fmul_rn(d, to_f32(weight[i]));
-            dx[row * cols + i] = from_f32<T>(r * fmaf(-hat, across, d - along));
+#pragma unroll 2
+        for (int64_t i = threadIdx.x * VEC; i < cols; i += 1024 * VEC) {
+            const P px = *reinterpret_cast<const P *>(xr + i), pd = *reinterpret_cast<const P *>(dr + i);
+            P w, q;
+            if (weight != nullptr) w = *reinterpret_cast<const P *>(weight + i);
+            float o[VEC];
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) {
+                float d = pd.get(k);
+                if (weight != nullptr) d = __fmul_rn(d, w.get(k));
+                o[k] = r * fmaf(-__fmul_rn(px.get(k) - m, r), across, d - along);
+            }
+            q.set(o);
+            *reinterpret_cast<P *>(dx + row * cols + i) = q;
         }
     }
 }
 
-// Column sums of long rows: a CTA takes 256 columns and one of gridDim.y slices of the rows.
-template <class T>
+// Column sums of long rows: a CTA takes 256 * VEC columns and one of gridDim.y slices of the rows.
+template <class T, int VEC>
 __global__ void __launch_bounds__(256)
     layer_norm_long_columns_kernel(const T *x, const float *mean, const float *rstd, const T *dy, int64_t rows, int64_t cols,
                                    float *partial) {
+    using P = Pack<T, VEC>;
     let_dependents_launch();
     dependency_wait();
-    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t c = ((int64_t)blockIdx.x * 256 + threadIdx.x) * VEC;
     if (c >= cols) return;
-    float w = 0.f, b = 0.f;
-#pragma unroll 8
+    float w[VEC], b[VEC];
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) w[k] = b[k] = 0.f;
+#pragma unroll 4
     for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
-        const float d = to_f32(dy[r * cols + c]);
-        w = fmaf(d, (to_f32(x[r * cols + c]) - mean[r]) * rstd[r], w);
-        b += d;
+        const P px = *reinterpret_cast<const P *>(x + r * cols + c), pd = *reinterpret_cast<const P *>(dy + r * cols + c);
+        const float m = mean[r], rs = rstd[r];
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+            const float d = pd.get(k);
+            w[k] = fmaf(d, __fmul_rn(px.get(k) - m, rs), w[k]);
+            b[k] += d;
+        }
     }
-    partial[(int64_t)blockIdx.y * 2 * cols + c] = w;
-    partial[(int64_t)blockIdx.y * 2 * cols + cols + c] = b;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+        partial[(int64_t)blockIdx.y * 2 * cols + c + k] = w[k];
+        partial[(int64_t)blockIdx.y * 2 * cols + cols + c + k] = b[k];
+    }
 }
 
 // ---- host ------------------------------------------------------------------------------------------
@@ -451,23 +479,47 @@ struct Backward {
     static constexpr int64_t kLastAdds = 16384;   // partial sums of each gradient that the last CTA adds
 };
 
-// The kernel whose registers hold a row: values a thread rounded up to a power of two, of a warp up to 1024 columns, then of a
-// CTA.  `MOST`: the most values a thread of a CTA may hold.
-template <int VEC, int MOST, class F>
-int by_columns(const F &f) {
+// The kernel whose registers hold a row.  With vectors as few threads as can hold it: a row of a warp needs no barrier, and what a
+// row of a CTA waits at its barriers other rows of the SM fill.  us, with 256 threads or more from 1024 columns on, and so: bf16
+// forward 32768 x 2048 95.6 and 50.1, 16384 x 4096 67.2 and 50.6, 8192 x 8192 73.2 and 53.8, backward 162 and 115.  Single values
+// would be many loads of few threads: f32 4093 x 2011 forward 17.8 with 256 threads, 24.1 with 128, backward 27.9 and 36.9.
+template <int VEC, class F>
+int forward_by_columns(const F &f) {
     const int64_t n = f.cols;
     if (VEC < 8 && n <= 32 * 4) return f.template run<VEC, 32, 4 / (VEC < 8 ? VEC : 1)>();
     if (n <= 32 * 8) return f.template run<VEC, 32, 8 / VEC>();
     if (n <= 32 * 16) return f.template run<VEC, 32, 16 / VEC>();
     if (n <= 32 * 32) return f.template run<VEC, 32, 32 / VEC>();
+    if constexpr (VEC > 1) {
+        if (n <= 32 * 64) return f.template run<VEC, 32, 64 / VEC>();
+        if (n <= 128 * 32) return f.template run<VEC, 128, 32 / VEC>();
+        if (n <= 256 * 32) return f.template run<VEC, 256, 32 / VEC>();
+        if (n <= 512 * 32) return f.template run<VEC, 512, 32 / VEC>();
+        return f.template run<VEC, 512, 64 / VEC>();
+    }
     if (n <= 256 * 8) return f.template run<VEC, 256, 8 / VEC>();
     if (n <= 256 * 16) return f.template run<VEC, 256, 16 / VEC>();
     if (n <= 512 * 16) return f.template run<VEC, 512, 16 / VEC>();
-    if constexpr (MOST > 16) {
-        if (n <= 1024 * 16) return f.template run<VEC, 1024, 16 / VEC>();
-        return f.template run<VEC, 1024, 32 / VEC>();
+    if (n <= 1024 * 16) return f.template run<VEC, 1024, 16 / VEC>();
+    return f.template run<VEC, 1024, 32 / VEC>();
+}
+// The sums of the columns take two more registers a value.
+template <int VEC, class F>
+int backward_by_columns(const F &f) {
+    const int64_t n = f.cols;
+    if (VEC < 8 && n <= 32 * 4) return f.template run<VEC, 32, 4 / (VEC < 8 ? VEC : 1)>();
+    if (n <= 32 * 8) return f.template run<VEC, 32, 8 / VEC>();
+    if (n <= 32 * 16) return f.template run<VEC, 32, 16 / VEC>();
+    if (n <= 32 * 32) return f.template run<VEC, 32, 32 / VEC>();
+    if constexpr (VEC == 8) {
+        if (n <= 128 * 16) return f.template run<VEC, 128, 16 / VEC>();
+        if (n <= 128 * 32) return f.template run<VEC, 128, 32 / VEC>();
+        return f.template run<VEC, 256, 32 / VEC>();
     }
-    return AG_ERR_UNSUPPORTED;
+    if (VEC > 1 && n <= 128 * 16) return f.template run<VEC, 128, 16 / VEC>();
+    if (n <= 256 * 8) return f.template run<VEC, 256, 8 / VEC>();
+    if (n <= 256 * 16) return f.template run<VEC, 256, 16 / VEC>();
+    return f.template run<VEC, 512, 16 / VEC>();
 }
 
 template <class T>
@@ -488,7 +540,7 @@ int forward(ag_device *dev, const T *x, const T *weight, const T *bias, int64_t 
                                 rows, cols, eps, y, mean, rstd);
     }
     const Forward<T> f = {dev, x, weight, bias, rows, cols, eps, y, mean, rstd};
-    return vectors<T>(cols, {x, weight, bias, y}) ? by_columns<16 / sizeof(T), 32>(f) : by_columns<1, 32>(f);
+    return vectors<T>(cols, {x, weight, bias, y}) ? forward_by_columns<16 / sizeof(T)>(f) : forward_by_columns<1>(f);
 }
 
 template <class T>
@@ -497,19 +549,21 @@ int backward(ag_device *dev, const T *x, const T *weight, const float *mean, con
     const Backward<T> f = {dev, x, weight, mean, rstd, dy, rows, cols, dx, beta, dweight, dbias};
     if (dx == nullptr && !f.sums()) return AG_OK;
     if (rows == 0) return f.sums() ? f.add_columns(0, {nullptr, nullptr, beta, dweight, dbias}) : AG_OK;
-    if (cols <= 512 * 16) return vectors<T>(cols, {x, weight, dy, dx}) ? by_columns<16 / sizeof(T), 16>(f) : by_columns<1, 16>(f);
+    if (cols <= 512 * 16) return vectors<T>(cols, {x, weight, dy, dx}) ? backward_by_columns<16 / sizeof(T)>(f) : backward_by_columns<1>(f);
+    const bool vec = vectors<T>(cols, {x, weight, dy, dx});
+    constexpr int V = 16 / sizeof(T);
     if (dx != nullptr) {
         const int64_t most = 2 * dev->sm_count;
-        AG_TRY(launch_dependent(dev, layer_norm_long_backward_kernel<T>, dim3((unsigned)(rows < most ? rows : most)), 1024, 0, x,
-                                weight, mean, rstd, dy, rows, cols, dx));
+        AG_TRY(launch_dependent(dev, vec ? layer_norm_long_backward_kernel<T, V> : layer_norm_long_backward_kernel<T, 1>,
+                                dim3((unsigned)(rows < most ? rows : most)), 1024, 0, x, weight, mean, rstd, dy, rows, cols, dx));
     }
     if (!f.sums()) return AG_OK;
-    const int64_t blocks = ceil_div(cols, 256), want = ceil_div((int64_t)8 * dev->sm_count, blocks);
+    const int64_t blocks = ceil_div(cols, 256 * (vec ? V : 1)), want = ceil_div((int64_t)8 * dev->sm_count, blocks);
     const int slices = (int)(want < rows ? want : rows);
     void *ws;
     AG_TRY(workspace(dev, (size_t)slices * 2 * cols * sizeof(float), &ws));
-    AG_TRY(launch_dependent(dev, layer_norm_long_columns_kernel<T>, dim3((unsigned)blocks, (unsigned)slices), 256, 0, x, mean, rstd,
-                            dy, rows, cols, (float *)ws));
+    AG_TRY(launch_dependent(dev, vec ? layer_norm_long_columns_kernel<T, V> : layer_norm_long_columns_kernel<T, 1>,
+                            dim3((unsigned)blocks, (unsigned)slices), 256, 0, x, mean, rstd, dy, rows, cols, (float *)ws));
     return f.add_columns(slices, {(float *)ws, nullptr, beta, dweight, dbias});
 }
 
