@@ -14,8 +14,8 @@
 // A backward group takes every `groups`-th row and adds dy * hat and dy of its columns in registers as it goes; the CTAs'
 // sums are added in the order of the CTAs, by the CTA that finishes last or, where there is more to add, by a second
 // kernel.  Longer rows take two kernels that read them again.
-// Of the measured copy bandwidth, 65536 x 1024: f32 forward 0.97 (85 us), backward 0.70 (177), bf16 0.86 (48) and 0.72 (86);
-// backward is near its instructions there, about twenty a value; 256 x 25088 f32 forward 0.65 (12 us, half a row an SM at a time).
+// Of the measured copy bandwidth, 65536 x 1024: f32 forward 0.97 (85 us), backward 0.91 (136), bf16 0.86 (48) and 0.72 (86: a
+// quarter of the warps, whose 128 registers hold row and sums); 256 x 25088 f32 forward 0.65 (12 us in L2, one row an SM at a time).
 //
 // Products that feed a sum are written as __fmul_rn or fmaf: left to the compiler, it fuses them one way in the loop for calls
 // that ask for the statistics, or for one gradient, and another way in the next, and the same values would give other bits.
@@ -495,7 +495,8 @@ int forward_by_columns(const F &f) {
         if (n <= 128 * 32) return f.template run<VEC, 128, 32 / VEC>();
         if (n <= 256 * 32) return f.template run<VEC, 256, 32 / VEC>();
         if (n <= 512 * 32) return f.template run<VEC, 512, 32 / VEC>();
-        return f.template run<VEC, 512, 64 / VEC>();
+        // f32 256 x 25088 from memory 17.1 us with 1024 threads, 20.1 with 512; bf16 2048 x 25088 60 and 46
+        return f.template run<VEC, VEC == 8 ? 512 : 1024, VEC == 8 ? 8 : 32 / VEC>();
     }
     if (n <= 256 * 8) return f.template run<VEC, 256, 8 / VEC>();
     if (n <= 256 * 16) return f.template run<VEC, 256, 16 / VEC>();
@@ -510,6 +511,9 @@ int backward_by_columns(const F &f) {
     if (VEC < 8 && n <= 32 * 4) return f.template run<VEC, 32, 4 / (VEC < 8 ? VEC : 1)>();
     if (n <= 32 * 8) return f.template run<VEC, 32, 8 / VEC>();
     if (n <= 32 * 16) return f.template run<VEC, 32, 16 / VEC>();
+    // f32, many rows: 128 registers a thread keep a third of the warps; us, 65536 x 1024 177 and 136, 1000 x 1024 9.1 and 15.9
+    // (bf16 86 and 116)
+    if (VEC == 4 && n > 512 && n <= 32 * 32 && f.rows >= 16384) return f.template run<VEC, 128, 8 / VEC>();
     if (n <= 32 * 32) return f.template run<VEC, 32, 32 / VEC>();
     if constexpr (VEC == 8) {
         if (n <= 128 * 16) return f.template run<VEC, 128, 16 / VEC>();
@@ -613,6 +617,10 @@ int ag_layer_norm_backward(ag_device *dev, ag_dtype dtype, const void *x, const 
     const int64_t es = (int64_t)dtype_size(dtype), n = rows * cols * es;
     AG_REQUIRE(!norm::overlap(dx, n, x, n) && !norm::overlap(dx, n, dy, n), AG_ERR_INVALID,
                "layer_norm: dx must not overlap x or dy");
+    const int64_t vector = cols * es;
+    AG_REQUIRE(!norm::overlap(dweight, vector, dbias, vector) && !norm::overlap(dx, n, dweight, vector) &&
+                   !norm::overlap(dx, n, dbias, vector),
+               AG_ERR_INVALID, "layer_norm: the gradients must not overlap");
     if (dtype == AG_F32)
         return norm::backward(dev, (const float *)x, (const float *)weight, mean, rstd, (const float *)dy, rows, cols, (float *)dx,
                               beta, (float *)dweight, (float *)dbias);

@@ -2,7 +2,9 @@
 //
 // With x = u / norm(u), as n x m with n <= m (the transpose of a taller u), a step is
 //   a = x x^T,  b = B a + C a a,  x <- A x + b x,   (A, B, C) = (3.4445, -4.7750, 2.0315),
-// which maps every singular value s to A s + B s^3 + C s^5 and keeps the singular vectors.
+// which maps every singular value s to A s + B s^3 + C s^5 and keeps the singular vectors.  muon_product.cuh has the steps; here
+// are the passes before them for large lists (25088 x 512 with its momentum: 42 and 50 us, 128 MB each), the choices by
+// size, and the entry points.
 #include <algorithm>
 #include <vector>
 
@@ -13,8 +15,11 @@ namespace muon {
 
 constexpr int64_t kMostShort = 16384, kMostLong = 1 << 20;
 constexpr int kMostMatrices = 4096, kMostSteps = 20;
+constexpr int64_t kMostRows = 4ll << 23;      // of the workspace of a launch with more than one matrix: 4 GiB
 constexpr int kMostParts = 2048;              // partial sums of squares of a matrix
-constexpr int64_t kInside = 1 << 20;          // values of a launch up to which its one kernel does everything
+// Values of a launch up to which its one kernel makes the planes too (LeNet5's weights 127.9 us, apart 129.8, one launch for
+// three).  Larger passes are bound by memory, which that kernel's eleven warps an SM do not keep busy.
+constexpr int64_t kInside = 1 << 20;
 
 // The CTA's matrix, of which it takes the `count(m)`-th piece.
 template <class F>
@@ -73,19 +78,20 @@ static int launch(ag_device *dev, const CUtensorMap &map, __half *planes, double
 
 template <class T>
 int run(ag_device *dev, const std::vector<Matrix> &matrices, const Rule &rule, int steps) {
-    for (size_t first = 0; first < matrices.size(); first += kGroup) {
+    int taken = 0;
+    for (size_t first = 0; first < matrices.size(); first += taken) {
         Group g = {};
-        g.n = (int)std::min<size_t>(kGroup, matrices.size() - first);
         g.steps = steps;
         g.rule = rule;
         int64_t space = 0;
         int parts = 0, blocks = 0;
         int64_t values = 0, tiles = 0;
-        for (int i = 0; i < g.n; ++i) {
-            Matrix &m = g.m[i];
-            m = matrices[first + i];
-            const int64_t n = std::min(m.rows, m.cols), wide = std::max(m.rows, m.cols);
+        for (; g.n < kGroup && first + g.n < matrices.size(); ++g.n) {
+            Matrix &m = g.m[g.n];
+            m = matrices[first + g.n];
+            const int64_t n = m.n(), wide = m.wide();
             m.squares = squares_from(m, steps, sizeof(T) == 2);
+            if (g.n > 0 && space + m.space(steps) > kMostRows) break;
             m.row = (int)std::min<int64_t>(space, INT32_MAX);
             space += m.space(steps);
             g.phases = std::max(g.phases, m.phases(steps));
@@ -96,8 +102,11 @@ int run(ag_device *dev, const std::vector<Matrix> &matrices, const Rule &rule, i
             values += n * wide;
             tiles += ceil_div(n, 128) * ceil_div(wide, 128);
         }
+        taken = g.n;
         AG_REQUIRE(space < (1ll << 31), AG_ERR_LIMIT, "newton_schulz: the matrices' workspace is too large");
         g.inside = values <= kInside;
+        // Tiles of 64 columns where wide ones would leave SMs idle: us, wide and narrow, f32 1024 x 1024 329 and 242, 512 x 512 230
+        // and 165, 1536 x 1024 331 and 313; beyond a tile an SM wide ones win (two 1024 x 1024 and 700 x 700 405 and 451).
         const bool narrow = tiles <= dev->sm_count;
         const size_t heads = (size_t)kGroup * kMostParts * sizeof(double), sums = (size_t)dev->sm_count * 128 * 128 * sizeof(float);
         void *ws;

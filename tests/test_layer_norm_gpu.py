@@ -398,6 +398,8 @@ def test_refusals(dev):
     assert b(dev._h, 0, p(x), None, None, p(m), p(x), 4, 8, p(flat), 0.0, None, None) == inv
     assert b(dev._h, 0, p(x), None, p(m), p(m), p(flat), 4, 8, p(flat), 0.0, None, None) == inv
     assert b(dev._h, 0, p(flat), None, p(m), p(m), p(x), 4, 8, p(flat) + 64, 0.0, None, None) == inv
+    assert b(dev._h, 0, p(x), None, p(m), p(m), p(x), 4, 8, None, 0.0, p(flat), p(flat) + 16) == inv
+    assert b(dev._h, 0, p(x), None, p(m), p(m), p(x), 4, 8, p(flat), 0.0, p(flat) + 64, None) == inv
     assert b(dev._h, 0, p(x), None, p(m), p(m), p(x), 4, 8, None, 0.0, None, None) == 0   # nothing asked for
 
 

@@ -105,6 +105,18 @@ def test_a_list_of_matrices(dev, dtype):
 
 
 @gpu
+def test_a_list_larger_than_one_workspace(dev):
+    """Matrices whose planes together are beyond the 4 GiB that a launch takes go in several."""
+    dev.set_guards(False)
+    g = torch.randn((4096, 8192), device=dev.torch_device, generator=torch.Generator("cuda").manual_seed(1)).bfloat16()
+    want, = dev.newton_schulz([g])
+    outs = dev.newton_schulz([g] * 9 + [g[:100, :200].contiguous()])
+    assert all(torch.equal(o, want) for o in outs[:8])
+    _close(outs[9], _polar64(g[:100, :200]), BF16)
+    _close(want[:, :64].contiguous(), _polar64(g)[:, :64], BF16)
+
+
+@gpu
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 @pytest.mark.parametrize("rows,cols", [(40, 60), (300, 200), (200, 1500)])
 @pytest.mark.parametrize("steps", [1, 2, 3, 7])
