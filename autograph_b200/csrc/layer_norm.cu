@@ -134,7 +134,8 @@ __global__ void __launch_bounds__(threads_of<G>())
                 if (bias != nullptr) b = *reinterpret_cast<const P *>(bias + col);
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) {
-                    o[i] = fmaf(__fmul_rn(p[c].get(i) - mean, rstd), weight != nullptr ? w.get(i) : 1.f, bias != nullptr ? b.get(i) : 0.f);
+                    o[i] = fmaf(__fmul_rn(p[c].get(i) - mean, rstd), weight != nullptr ? w.get(i) : 1.f,
+                                bias != nullptr ? b.get(i) : 0.f);
                 }
                 P q;
                 q.set(o);
@@ -553,7 +554,8 @@ int backward(ag_device *dev, const T *x, const T *weight, const float *mean, con
     const Backward<T> f = {dev, x, weight, mean, rstd, dy, rows, cols, dx, beta, dweight, dbias};
     if (dx == nullptr && !f.sums()) return AG_OK;
     if (rows == 0) return f.sums() ? f.add_columns(0, {nullptr, nullptr, beta, dweight, dbias}) : AG_OK;
-    if (cols <= 512 * 16) return vectors<T>(cols, {x, weight, dy, dx}) ? backward_by_columns<16 / sizeof(T)>(f) : backward_by_columns<1>(f);
+    if (cols <= 512 * 16)
+        return vectors<T>(cols, {x, weight, dy, dx}) ? backward_by_columns<16 / sizeof(T)>(f) : backward_by_columns<1>(f);
     const bool vec = vectors<T>(cols, {x, weight, dy, dx});
     constexpr int V = 16 / sizeof(T);
     if (dx != nullptr) {

@@ -389,7 +389,8 @@ __device__ __forceinline__ Job make_job(const Matrix &m, int kind, int step, int
     const int at_x = kind == kFinish ? m.squares % 2 : step % 2;   // x moves with every step on x itself
     const Stored x = m.x(at_x), a = m.square(0);
     // p and the product q of all p so far change places; the first q is the first p
-    const Stored p = m.square(1 + step % 2), q_old = step < 2 ? m.square(1) : m.square(4 + step % 2), q_new = m.square(4 + (step + 1) % 2);
+    const Stored p = m.square(1 + step % 2), q_old = step < 2 ? m.square(1) : m.square(4 + step % 2);
+    const Stored q_new = m.square(4 + (step + 1) % 2);
     const float scale_q = kScaleB * exp2f(-2.f * (float)step), scale_old = kScaleB * exp2f(-2.f * (float)(step - 1));
     Job j;
     j.planes = kind <= kApply && step < m.squares ? planes_of(sizeof(T) == 2, n, step, steps) : 2;
