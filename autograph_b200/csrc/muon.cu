@@ -48,8 +48,8 @@ __global__ void __launch_bounds__(256) split_kernel(const __grid_constant__ Grou
 }
 
 // First step on x x^T alone (muon_product.cuh).  Counted in products of planes of an n x n matrix, for x of r times its size:
-// f32 22.5 r + 7.5 on x throughout, 13.5 r + 16.5 from the third step on; bf16 13.5 r + 4.5 (some steps take one product of
-// planes), 6 r + 20 from the second.  At most five steps: f16 holds no more of q's range.
+// 22.5 r + 7.5 on x throughout, 13.5 r + 16.5 from the third step on (f32), 9 r + 21 from the second (bf16).  At most five
+// steps: f16 holds no more of q's range.
 static int squares_from(const Matrix &m, int steps, bool bf16) {
     if (m.n() < 128 || m.wide() < 2 * m.n()) return steps;
     return std::min(steps, std::max(bf16 ? 1 : 2, steps - 5));

@@ -2,9 +2,11 @@
 // phase, D = c0 * (P . Q) + c1 * E on tcgen05, with a barrier of the whole grid between two phases.
 //
 // Matrices live in one workspace as f16 planes.  A value x is held as hi + lo, hi = f16(x * 2^k) and lo = f16 of what
-// that leaves: 22 bits, of which a product takes hi.hi + hi.lo + lo.hi (what is dropped is 2^-24 of a product at most, as
-// f32's own rounding), or hi.hi alone where eleven bits are enough.  The scales 2^k are fixed, because the values are
-// bounded: the singular values of every x of the iteration stay below 1.21.
+// that leaves: 22 bits, of which a product takes hi.hi + hi.lo + lo.hi.  lo is at most 2^-11 of hi, so what is dropped is at
+// most 2^-22 of a product, and lo's own rounding 2^-22 of a value.  bf16 results take the same products: a step's map of the
+// singular values has slopes of A at zero, -1.6 at 0.87 and 4 at 1.21, so that what a step rounds off stays or grows.  hi.hi
+// alone in three steps of five was 1.0e-3 of the result off beside its rounding of 1.7e-3, in all but three of twenty 1e-2.  The
+// scales 2^k are fixed, because the values are bounded: the singular values of every x of the iteration stay below 1.21.
 //
 // A matrix of R x C is stored in panels of 64 columns, [C / 64][Rp][64] with Rp = R rounded up to 128 and zeros in the
 // padding, so that a panel's rows are 128 bytes: the whole workspace is one matrix of 128-byte rows behind one tensor map,
@@ -81,7 +83,6 @@ struct Job {
     int steps;         // 64-k steps
     int symmetric;     // D is: only tiles on and above the diagonal are computed
     int has_e, final;
-    int planes;        // of each operand: 2 for hi.hi + hi.lo + lo.hi, 1 for hi.hi
     float c0, c1;
     float diagonal;    // added to D's
 };
@@ -343,18 +344,9 @@ __device__ __forceinline__ void split_tile(const Matrix &m, const Rule &r, int b
 // tile each, and one plans the next phase.
 constexpr int kEpilogue = 8, kPlanner = 2 + kEpilogue, kThreads = (kPlanner + 1) * 32;
 constexpr int kBox = 64 * 64 * 2;          // bytes of a box of the tensor map
-// A stage: both planes of 64 k, or the upper one of 128, of 128 rows of P and up to 128 of Q.
+// A stage: both planes of 64 k of 128 rows of P and up to 128 of Q.
 constexpr int kStage = 8 * kBox, kStages = 3;
 constexpr int kSmem = kStages * kStage + 1024;
-
-// Products of planes of a step.  bf16 results: the products of the last step and of those before the last three are of the
-// planes' upper halves alone.  What an early step rounds off is later drawn to one with the singular values; what the last
-// one does is 2^-12 of its operands and not multiplied any more.  Short sides average too little for that, and their
-// products cost nothing.
-__device__ __forceinline__ int planes_of(bool bf16, int n, int step, int steps) {
-    const int left = steps - 1 - step;
-    return bf16 && n >= 128 && (left == 0 || left > 2) ? 1 : 2;
-}
 
 // The products of a matrix, phase by phase.  On x itself a step is
 //   kGram a = x x^T, kPoly b = B a + C a a, kApply x = A x + b x.
@@ -393,7 +385,6 @@ __device__ __forceinline__ Job make_job(const Matrix &m, int kind, int step, int
     const Stored q_new = m.square(4 + (step + 1) % 2);
     const float scale_q = kScaleB * exp2f(-2.f * (float)step), scale_old = kScaleB * exp2f(-2.f * (float)(step - 1));
     Job j;
-    j.planes = kind <= kApply && step < m.squares ? planes_of(sizeof(T) == 2, n, step, steps) : 2;
     j.final = 0;
     j.M = n;
     j.N = n;
@@ -712,8 +703,8 @@ __device__ __forceinline__ bool run_phase(const Cta &t, int phase, int barrier, 
         for (int w = blockIdx.x; w < units; w += gridDim.x) {
             const Item it = w == (int)blockIdx.x ? first : find_item<BN>(*plan, w);
             const Job &j = plan->job[it.copy][it.matrix];
-            const bool two = j.planes == 2, q_mn = j.q_mn;
-            const int per = two ? 1 : 2, count = (it.k1 - it.k0 + per - 1) / per;
+            const bool q_mn = j.q_mn;
+            const int count = it.k1 - it.k0;
             // rows of a step's boxes, and from one to the next
             const int p_base = j.p.row + it.m0, p_plane = j.p.plane, p_step = j.p.rp;
             const int q_base = j.q.row + (q_mn ? it.n0 / 64 * j.q.rp : it.n0), q_plane = j.q.plane, q_step = q_mn ? 64 : j.q.rp;
@@ -726,11 +717,10 @@ __device__ __forceinline__ bool run_phase(const Cta &t, int phase, int barrier, 
                         break;
                     }
                     const uint32_t bar = t.full + at_stage * 8, dst = t.stages + at_stage * kStage;
-                    const int k = it.k0 + c * per, halves = two || k + 1 < it.k1 ? 2 : 1;
-                    mbar_arrive_expect_tx(bar, halves * HALF);
-                    for (int h = 0; h < halves; ++h) {
-                        const int kk = two ? k : k + h, p_row = p_base + (two ? h * p_plane : 0) + kk * p_step;
-                        const int q_row = q_base + (two ? h * q_plane : 0) + kk * q_step;
+                    const int k = it.k0 + c;
+                    mbar_arrive_expect_tx(bar, 2 * HALF);
+                    for (int h = 0; h < 2; ++h) {
+                        const int p_row = p_base + h * p_plane + k * p_step, q_row = q_base + h * q_plane + k * q_step;
                         const uint32_t to = dst + h * HALF;
                         tma_load_2d(to, t.map, bar, 0, p_row);
                         tma_load_2d(to + kBox, t.map, bar, 0, p_row + 64);
@@ -746,8 +736,8 @@ __device__ __forceinline__ bool run_phase(const Cta &t, int phase, int barrier, 
         for (int w = blockIdx.x; w < units; w += gridDim.x) {
             const Item it = w == (int)blockIdx.x ? first : find_item<BN>(*plan, w);
             const Job &j = plan->job[it.copy][it.matrix];
-            const bool two = j.planes == 2, q_mn = j.q_mn;
-            const int per = two ? 1 : 2, count = (it.k1 - it.k0 + per - 1) / per;
+            const bool q_mn = j.q_mn;
+            const int count = it.k1 - it.k0;
             if (elect_one()) {
                 const uint32_t idesc = half_idesc(q_mn, 128, BN);
                 const uint32_t q_step = q_mn ? 16 * 128 : 32, q_lbo = q_mn ? kBox : 0;
@@ -769,22 +759,14 @@ __device__ __forceinline__ bool run_phase(const Cta &t, int phase, int barrier, 
                                   make_smem_desc(base + hq * HALF + 2 * kBox + i * q_step, q_lbo, 1024), idesc, add ? 1u : 0u);
                     };
                     const bool more = c % kAccStages != 0;
-                    if (two) {
-                        // the small products first: what an addition cuts off is a part of the sum so far
+                    // the small products first: what an addition cuts off is a part of the sum so far
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            mma(0, 1, i, more || i > 0);
-                            mma(1, 0, i, true);
-                        }
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) mma(0, 0, i, true);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) mma(0, 0, i, more || i > 0);
-                        if (it.k0 + 2 * c + 1 < it.k1)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) mma(1, 1, i, true);
+                    for (int i = 0; i < 4; ++i) {
+                        mma(0, 1, i, more || i > 0);
+                        mma(1, 0, i, true);
                     }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) mma(0, 0, i, true);
                     umma_commit(t.empty + at_stage * 8);
                     if ((c + 1) % kAccStages == 0 || c + 1 == count) umma_commit(t.acc_full + acc % 2 * 8);
                 }
@@ -797,8 +779,7 @@ __device__ __forceinline__ bool run_phase(const Cta &t, int phase, int barrier, 
         for (int w = blockIdx.x; w < units; w += gridDim.x) {
             const Item it = w == (int)blockIdx.x ? first : find_item<BN>(*plan, w);
             const Job &j = plan->job[it.copy][it.matrix];
-            const int per = j.planes == 2 ? 1 : 2, count = (it.k1 - it.k0 + per - 1) / per;
-            const int reads = (count + kAccStages - 1) / kAccStages;
+            const int reads = (it.k1 - it.k0 + kAccStages - 1) / kAccStages;
             finish_tile<T, BN>(t, it, j, w, splits, accs, reads);
             accs += reads;
         }

@@ -128,6 +128,26 @@ def test_steps(dev, rows, cols, dtype, steps):
     assert off <= _tol(dtype) * max(1.0, steps / 5)
 
 
+def _beside_the_rounding(dev, g, steps):
+    """The error of a bf16 result relative to that of the 64-bit result rounded to bf16.  Where the computation's error is
+    independent of the rounding's and less than 0.32 of it, this is below 1.05."""
+    want = _polar64(g, steps)
+    off = (dev.newton_schulz([g], steps=steps)[0].double() - want).norm()
+    return off / (want.bfloat16().double() - want).norm()
+
+
+@gpu
+@pytest.mark.parametrize("steps", [1, 5, 8, 10, 20])
+@pytest.mark.parametrize("rows,cols,rank", [(128, 128, None), (256, 256, None), (300, 257, None), (1024, 1024, None),
+                                            (300, 500, 5), (500, 300, 40)])
+def test_bf16_results_are_as_good_as_their_rounding(dev, rows, cols, rank, steps):
+    """Products of 22-bit values perturb x by about 1e-7 a step, and its map's slopes (A at zero, -1.6 to 4 around one)
+    make that 1e-4 at most in twenty steps: far less than 0.32 of the rounding's 1.65e-3.  What bf16 left of a low rank's zeros
+    are singular values of some 1e-4 of the largest, which grow as what rounds them off does."""
+    g = _gradient(rows, cols, 7, batch=rank).bfloat16().to(dev.torch_device)
+    assert _beside_the_rounding(dev, g, steps) <= 1.05
+
+
 @gpu
 @pytest.mark.parametrize("rows,cols", [(96, 200), (300, 500), (500, 300), (256, 1300)])
 @pytest.mark.parametrize("rank", [1, 2, 5, 40])
