@@ -47,12 +47,13 @@ __global__ void __launch_bounds__(256) split_kernel(const __grid_constant__ Grou
     split_tile<T, 256>(g.m[i], g.rule, block, inv, planes, tile);
 }
 
-// First step on x x^T alone (muon_product.cuh).  Counted in products of planes of an n x n matrix, for x of r times its size:
-// 22.5 r + 7.5 on x throughout, 13.5 r + 16.5 from the third step on (f32), 9 r + 21 from the second (bf16).  At most five
-// steps: f16 holds no more of q's range.
+// First step on x x^T alone (muon_product.cuh): the last two, for bf16 results the last three, but not the first two.  Counted in
+// products of planes of an n x n matrix, for x of r times its size, five steps are 22.5 r + 7.5 on x throughout, 18 r + 12 with
+// two on x x^T, 13.5 r + 16.5 with three.  us, f32, two and three: 25088 x 512 with three small ones 636 and 548, four of 1024 x 4096
+// 1025 and 892, 509 x 1531 twice and 777 x 1009 392 and 364.
 static int squares_from(const Matrix &m, int steps, bool bf16) {
     if (m.n() < 128 || m.wide() < 2 * m.n()) return steps;
-    return std::min(steps, std::max(bf16 ? 1 : 2, steps - 5));
+    return std::min(steps, std::max(2, steps - (bf16 ? 3 : 2)));
 }
 
 template <class T, int BN>

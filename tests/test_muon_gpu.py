@@ -149,6 +149,25 @@ def test_bf16_results_are_as_good_as_their_rounding(dev, rows, cols, rank, steps
 
 
 @gpu
+@pytest.mark.parametrize("steps", [3, 5, 6, 7, 8, 9])
+@pytest.mark.parametrize("rows,cols,rank", [(500, 1300, 40), (1300, 500, 5), (256, 1300, 1), (512, 2048, 100)])
+def test_low_ranks_of_long_matrices(dev, rows, cols, rank, steps):
+    """Gradients of few examples in bf16, whose rounding leaves singular values of some 1e-4 of the largest.  f32: no further from
+    64 bits than twice the same steps in f32 products, whose errors are of the same kind and size and may lie otherwise."""
+    g = _gradient(rows, cols, 7, batch=rank).bfloat16().to(dev.torch_device)
+    want = _polar64(g, steps)
+    x = g.float().T if rows > cols else g.float()
+    x = x / x.norm()
+    for _ in range(steps):
+        a = x @ x.T
+        x = A * x + (B * a + C * (a @ a)) @ x
+    plain = ((x.T if rows > cols else x).double() - want).norm()
+    off = (dev.newton_schulz([g.float()], steps=steps)[0].double() - want).norm()
+    assert off <= 2 * plain
+    assert _beside_the_rounding(dev, g, steps) <= 1.05
+
+
+@gpu
 @pytest.mark.parametrize("rows,cols", [(96, 200), (300, 500), (500, 300), (256, 1300)])
 @pytest.mark.parametrize("rank", [1, 2, 5, 40])
 def test_rank_deficient(dev, rows, cols, rank):
