@@ -149,6 +149,16 @@ def test_bf16_results_are_as_good_as_their_rounding(dev, rows, cols, rank, steps
 
 
 @gpu
+@pytest.mark.parametrize("steps", [5, 9, 20])
+@pytest.mark.parametrize("rows,cols,rank", [(1000, 2100, 5), (2000, 4100, 30), (2048, 2048, None)])
+def test_long_sums_of_bf16_results(dev, rows, cols, rank, steps):
+    """Sums over thousands of values, in pieces of 48 additions that are cut off by up to 2^-23 each: 3e-6 of x a step on
+    average, which grows like the roundings to a few 1e-4 in twenty steps."""
+    g = _gradient(rows, cols, 7, batch=rank).bfloat16().to(dev.torch_device)
+    assert _beside_the_rounding(dev, g, steps) <= 1.05
+
+
+@gpu
 @pytest.mark.parametrize("steps", [3, 5, 6, 7, 8, 9])
 @pytest.mark.parametrize("rows,cols,rank", [(500, 1300, 40), (1300, 500, 5), (256, 1300, 1), (512, 2048, 100)])
 def test_low_ranks_of_long_matrices(dev, rows, cols, rank, steps):
