@@ -84,13 +84,23 @@ __device__ __forceinline__ void group_sum(float (&v)[N], float *scratch) {
 template <int G>
 constexpr int threads_of() { return G == 32 ? 256 : G; }
 
+// From the sums of the differences from a first mean, and of their squares: the mean, put right by what the differences leave, and
+// 1 / sqrt(variance + eps).  The first mean is off by the roundings of a sum of n values, 1e-5 of it for 25088 equal ones; what
+// these differences leave is off by the same share of them, so that of equal values the mean is that value and y is the bias.
+// us with and without: bf16 65536 x 1024 54.9 and 51.8, f32 256 x 25088 18.1 and 17.1.
+__device__ __forceinline__ float finish_statistics(const float (&e)[2], float n, float eps, float &mean) {
+    const float left = __fdiv_rn(e[0], n), var = fmaf(-left, left, __fdiv_rn(e[1], n));
+    mean += left;
+    return 1.f / sqrtf((var < 0.f ? 0.f : var) + eps);   // NaN stays
+}
+
 // Rows in registers: NC packs of VEC values a thread.
 template <class T, int VEC, int G, int NC>
 __global__ void __launch_bounds__(threads_of<G>())
     layer_norm_kernel(const T *x, const T *weight, const T *bias, int64_t rows, int cols, float eps, T *y, float *mean_out,
                       float *rstd_out) {
     using P = Pack<T, VEC>;
-    __shared__ float scratch[32];
+    __shared__ float scratch[64];
     let_dependents_launch();
     dependency_wait();
     constexpr int GROUPS = threads_of<G>() / G;
@@ -111,18 +121,19 @@ __global__ void __launch_bounds__(threads_of<G>())
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) s[0] += p[c].get(i);
         group_sum<G>(s, scratch);
-        const float mean = __fdiv_rn(s[0], n);   // of equal values, that value
-        s[0] = 0.f;
+        float mean = __fdiv_rn(s[0], n);
+        float e[2] = {0.f, 0.f};
 #pragma unroll
         for (int c = 0; c < NC; ++c)
             if ((c * G + t) * VEC < cols)
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) {
                     const float d = p[c].get(i) - mean;
-                    s[0] = fmaf(d, d, s[0]);
+                    e[0] += d;
+                    e[1] = fmaf(d, d, e[1]);
                 }
-        group_sum<G>(s, scratch);
-        const float rstd = 1.f / sqrtf(__fdiv_rn(s[0], n) + eps);
+        group_sum<G>(e, scratch);
+        const float rstd = finish_statistics(e, n, eps, mean);
         T *yr = y + row * cols;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
@@ -154,7 +165,7 @@ template <class T>
 __global__ void __launch_bounds__(1024)
     layer_norm_long_kernel(const T *x, const T *weight, const T *bias, int64_t rows, int64_t cols, float eps, T *y,
                            float *mean_out, float *rstd_out) {
-    __shared__ float scratch[32];
+    __shared__ float scratch[64];
     let_dependents_launch();
     dependency_wait();
     for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
@@ -163,15 +174,16 @@ __global__ void __launch_bounds__(1024)
 #pragma unroll 8
         for (int64_t i = threadIdx.x; i < cols; i += 1024) s[0] += to_f32(xr[i]);
         group_sum<1024>(s, scratch);
-        const float mean = s[0] / (float)cols;
-        s[0] = 0.f;
+        float mean = __fdiv_rn(s[0], (float)cols);
+        float e[2] = {0.f, 0.f};
 #pragma unroll 8
         for (int64_t i = threadIdx.x; i < cols; i += 1024) {
-            const float c = to_f32(xr[i]) - mean;
-            s[0] = fmaf(c, c, s[0]);
+            const float d = to_f32(xr[i]) - mean;
+            e[0] += d;
+            e[1] = fmaf(d, d, e[1]);
         }
-        group_sum<1024>(s, scratch);
-        const float rstd = 1.f / sqrtf(s[0] / (float)cols + eps);
+        group_sum<1024>(e, scratch);
+        const float rstd = finish_statistics(e, (float)cols, eps, mean);
 #pragma unroll 4
         for (int64_t i = threadIdx.x; i < cols; i += 1024) {
             const float w = weight != nullptr ? to_f32(weight[i]) : 1.f, b = bias != nullptr ? to_f32(bias[i]) : 0.f;

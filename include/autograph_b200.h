@@ -464,11 +464,12 @@ typedef struct ag_polar_matrix {
  * x <- 3.4445 x - 4.7750 (x x^T) x + 2.0315 (x x^T)^2 x from x = g / norm(g) (Frobenius norm; the
  * shorter side multiplies), which takes the singular values of g / norm(g) to about one.  A
  * matrix of zeros gives zeros; one that holds a value that is not finite gives NaN.  Between the
- * steps values are held in 22 bits, whatever the dtype: the error of
- * an AG_BF16 result is within 5 % of its rounding's.  What rounding makes of singular values that are
- * exactly zero grows up to 3.4445-fold a step, as it does in f32 products: a result of low rank is up
- * to 1e-4 off after five steps and 2e-2 after ten, whatever the dtype.  steps in 1..20, n in 0..4096, the shorter side in 1..16384, the longer up to 2^20 and
- * fewer than 2^31 values per matrix; no o overlaps another matrix. */
+ * steps values are held in 22 bits, whatever the dtype: the error of an AG_BF16 result is within 5 %
+ * of its rounding's.  What rounding makes of singular values that are exactly zero grows up to
+ * 3.4445-fold a step, as it does in f32 products: a result of low rank is up to 1e-4 off after five
+ * steps and 2e-2 after ten, whatever the dtype.  steps in 1..20, n in 0..4096, the shorter side in
+ * 1..16384, the longer up to 2^20 and fewer than 2^31 values per matrix; no o overlaps another
+ * matrix. */
 AG_API int ag_newton_schulz(ag_device *dev, ag_dtype dtype, int32_t n,
                             const ag_polar_matrix *matrices, int32_t steps);
 

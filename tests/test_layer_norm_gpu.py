@@ -5,6 +5,7 @@ runs of at most r and then as a tree is off by at most (r + 20) u sum|x|, and ev
 at most n / 32 for the kernels' 32 or more partial sums of a row, and rows / 8 + 8 for a column's.
 """
 import ctypes
+import math
 
 import numpy as np
 import pytest
@@ -258,6 +259,42 @@ def test_constant_rows_and_far_means(dev, cols):
     y, mean, rstd = dev.layer_norm_keep(far)
     _check_forward(far, None, None, y, mean, rstd)
     assert (rstd > 0.8).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("cols", [5, 84, 1000, 2011, 4096, 8190, 25088, 70001])
+def test_rows_of_one_value(dev, cols, dtype):
+    """Values of full mantissas, whose sums are rounded.  A first mean m is off by at most (cols / 32 + 22) u of c, so that
+    c - m is exact; the mean of these equal differences is off by the same share of them, less than u / 4 of c, and added to
+    m gives c.  The variance is then zero up to that share of (c - m)^2."""
+    c = torch.cat([torch.tensor([1000.1, 1 / 3, 1234.567, -777.77, 1e-3, 3e7]),
+                   500 + 1500 * torch.rand(58, generator=torch.Generator().manual_seed(cols))])
+    x = c.to(dtype).to(dev.torch_device)[:, None].expand(64, cols).contiguous()
+    _, w, b, _ = _inputs(dev, 1, cols, dtype, seed=91)
+    y, mean, rstd = dev.layer_norm_keep(x, w, b)
+    assert torch.equal(mean, x[:, 0].float()) and torch.equal(y, b.expand(64, cols))
+    run = (cols / 32 + 24) * U
+    var = 4 * run * (run * x[:, 0].double()).square()
+    want = 1 / math.sqrt(EPS)
+    assert ((rstd.double() - want).abs() <= want * (4 * U + var / EPS / 2)).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("rows,cols", [(9, 84), (9, 1000), (9, 2011), (5, 25088), (3, 70001)])
+@pytest.mark.parametrize("shift", [0.0, 30.0, 1000.1])
+def test_far_means_are_rounded_once(dev, rows, cols, dtype, shift):
+    """The mean is off by its own rounding, that of the differences it is put right by (u of each) and that of their sum,
+    (cols / 32 + 24) u of their size, however far it is.  A first mean m that is off by q = (cols / 32 + 22) u |mean| adds
+    q to the differences."""
+    x = _rand((rows, cols), 7, 1.0, shift).to(dtype).to(dev.torch_device)
+    y, mean, rstd = dev.layer_norm_keep(x)
+    _check_forward(x, None, None, y, mean, rstd)
+    x = x.double()
+    exact = x.mean(1)
+    spread = (x - exact[:, None]).abs().mean(1) + (cols / 32 + 22) * U * x.abs().mean(1)
+    assert ((mean.double() - exact).abs() <= U * exact.abs() + (cols / 32 + 25) * U * spread + 1e-45).all()
 
 
 @gpu
