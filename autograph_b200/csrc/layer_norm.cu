@@ -594,10 +594,26 @@ static int check_sizes(ag_dtype dtype, int64_t rows, int64_t cols) {
     return AG_OK;
 }
 
-// Whether two ranges of `na` and `nb` bytes share a byte.
-static bool overlap(const void *a, int64_t na, const void *b, int64_t nb) {
-    const uintptr_t p = (uintptr_t)a, q = (uintptr_t)b;
-    return a != nullptr && b != nullptr && p < q + (uintptr_t)nb && q < p + (uintptr_t)na;
+// An operand of a call: its bytes, none where it is null.
+struct Range {
+    const void *p;
+    int64_t bytes;
+};
+
+// Refuses results that share a byte with another operand: rows are written while others' operands are still read.
+static int check_overlap(std::initializer_list<Range> results, std::initializer_list<Range> inputs) {
+    auto overlap = [](const Range &a, const Range &b) {
+        const uintptr_t p = (uintptr_t)a.p, q = (uintptr_t)b.p;
+        return a.p != nullptr && b.p != nullptr && a.bytes > 0 && b.bytes > 0 && p < q + (uintptr_t)b.bytes &&
+               q < p + (uintptr_t)a.bytes;
+    };
+    for (auto r = results.begin(); r != results.end(); ++r) {
+        for (const Range &i : inputs)
+            AG_REQUIRE(!overlap(*r, i), AG_ERR_INVALID, "layer_norm: a result overlaps an operand");
+        for (auto other = r + 1; other != results.end(); ++other)
+            AG_REQUIRE(!overlap(*r, *other), AG_ERR_INVALID, "layer_norm: the results must not overlap");
+    }
+    return AG_OK;
 }
 
 }  // namespace norm
@@ -613,8 +629,10 @@ int ag_layer_norm_forward(ag_device *dev, ag_dtype dtype, const void *x, const v
     AG_TRY(norm::check_sizes(dtype, rows, cols));
     AG_REQUIRE(eps > 0.f && eps <= 3.4e38f, AG_ERR_INVALID, "layer_norm: eps must be positive and finite");
     AG_REQUIRE(rows == 0 || (x && y), AG_ERR_INVALID, "layer_norm: null pointer");
-    const int64_t n = rows * cols * (int64_t)dtype_size(dtype);
-    AG_REQUIRE(x == y || !norm::overlap(x, n, y, n), AG_ERR_INVALID, "layer_norm: y must be x or not overlap it");
+    const int64_t es = (int64_t)dtype_size(dtype), n = rows * cols * es;
+    // y may be x: a row is read before it is written
+    AG_TRY(norm::check_overlap({{y, n}, {mean, rows * 4}, {rstd, rows * 4}},
+                               {{x == y ? nullptr : x, n}, {weight, cols * es}, {bias, cols * es}}));
     if (dtype == AG_F32)
         return norm::forward(dev, (const float *)x, (const float *)weight, (const float *)bias, rows, cols, eps, (float *)y, mean,
                              rstd);
@@ -629,12 +647,8 @@ int ag_layer_norm_backward(ag_device *dev, ag_dtype dtype, const void *x, const 
     AG_TRY(norm::check_sizes(dtype, rows, cols));
     AG_REQUIRE(rows == 0 || (x && mean && rstd && dy), AG_ERR_INVALID, "layer_norm: null pointer");
     const int64_t es = (int64_t)dtype_size(dtype), n = rows * cols * es;
-    AG_REQUIRE(!norm::overlap(dx, n, x, n) && !norm::overlap(dx, n, dy, n), AG_ERR_INVALID,
-               "layer_norm: dx must not overlap x or dy");
-    const int64_t vector = cols * es;
-    AG_REQUIRE(!norm::overlap(dweight, vector, dbias, vector) && !norm::overlap(dx, n, dweight, vector) &&
-                   !norm::overlap(dx, n, dbias, vector),
-               AG_ERR_INVALID, "layer_norm: the gradients must not overlap");
+    AG_TRY(norm::check_overlap({{dx, n}, {dweight, cols * es}, {dbias, cols * es}},
+                               {{x, n}, {dy, n}, {weight, cols * es}, {mean, rows * 4}, {rstd, rows * 4}}));
     if (dtype == AG_F32)
         return norm::backward(dev, (const float *)x, (const float *)weight, mean, rstd, (const float *)dy, rows, cols, (float *)dx,
                               beta, (float *)dweight, (float *)dbias);

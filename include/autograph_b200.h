@@ -390,7 +390,7 @@ AG_API int ag_bias_grad(ag_device *dev, ag_dtype dtype, const void *x, int64_t r
 
 /* Per row: mean = sum(x) / cols, rstd = 1 / sqrt(sum((x - mean)^2) / cols + eps),
  * y = (x - mean) * rstd * weight + bias.  mean and rstd [rows] (f32) are what the backward pass
- * reads; either may be NULL.  eps > 0.  y may be x, and must not overlap it otherwise. */
+ * reads; either may be NULL.  eps > 0.  y may be x; otherwise no result overlaps another operand. */
 AG_API int ag_layer_norm_forward(ag_device *dev, ag_dtype dtype, const void *x, const void *weight,
                                  const void *bias, int64_t rows, int64_t cols, float eps, void *y,
                                  float *mean, float *rstd);
@@ -399,7 +399,8 @@ AG_API int ag_layer_norm_forward(ag_device *dev, ag_dtype dtype, const void *x, 
  * dx = rstd * (d - sum(d) / cols - hat * sum(d * hat) / cols),
  * dweight = beta * dweight + sum over rows of dy * hat, dbias = beta * dbias + sum over rows of
  * dy (beta = 1 accumulates, beta = 0 does not read what was there; as in
- * ag_conv2_backward_weight).  dx, dweight and dbias may each be NULL; dx must not overlap x or dy.
+ * ag_conv2_backward_weight).  dx, dweight and dbias may each be NULL; none overlaps another
+ * operand.
  * The sums over rows are added in the same order on every call of the same sizes. */
 AG_API int ag_layer_norm_backward(ag_device *dev, ag_dtype dtype, const void *x, const void *weight,
                                   const float *mean, const float *rstd, const void *dy,

@@ -440,6 +440,53 @@ def test_refusals(dev):
     assert b(dev._h, 0, p(x), None, p(m), p(m), p(x), 4, 8, None, 0.0, None, None) == 0   # nothing asked for
 
 
+@gpu
+def test_results_that_overlap_operands_are_refused(dev):
+    """Rows are written while the operands of others are still read.  Nothing is launched: the operands keep their values."""
+    f, b, inv = ag.lib().ag_layer_norm_forward, ag.lib().ag_layer_norm_backward, ag._capi.AG_ERR_INVALID
+    store = torch.ones(400, device=dev.torch_device)
+    p = lambda i: store.data_ptr() + 4 * i
+    # [4, 8] x at 0, y at 40, weight at 80, bias at 90, mean at 100, rstd at 110, apart from each other
+    at = dict(x=0, y=40, weight=80, bias=90, mean=100, rstd=110)
+    size = dict(x=32, y=32, weight=8, bias=8, mean=4, rstd=4)
+
+    def forward(**moved):
+        a = {**at, **moved}
+        return f(dev._h, 0, p(a["x"]), p(a["weight"]), p(a["bias"]), 4, 8, EPS, p(a["y"]), p(a["mean"]), p(a["rstd"]))
+    for result in ("y", "mean", "rstd"):
+        for other in at:
+            if other == result:
+                continue
+            # on its last value, and with the result's last value on its first
+            places = [at[other] + size[other] - 1, at[other] - size[result] + 1]
+            for place in places:
+                if place >= 0:
+                    assert forward(**{result: place}) == inv, (result, other, place)
+    assert forward(y=1) == inv
+    at = dict(x=0, dy=40, weight=80, mean=100, rstd=110, dx=120, dweight=160, dbias=170)
+    size = dict(x=32, dy=32, weight=8, mean=4, rstd=4, dx=32, dweight=8, dbias=8)
+
+    def backward(**moved):
+        a = {**at, **moved}
+        return b(dev._h, 0, p(a["x"]), p(a["weight"]), p(a["mean"]), p(a["rstd"]), p(a["dy"]), 4, 8, p(a["dx"]), 0.0,
+                 p(a["dweight"]), p(a["dbias"]))
+    for result in ("dx", "dweight", "dbias"):
+        for other in at:
+            if other == result:
+                continue
+            for place in (at[other] + size[other] - 1, at[other] - size[result] + 1):
+                if place >= 0:
+                    assert backward(**{result: place}) == inv, (result, other, place)
+    dev.wait()
+    assert (store == 1).all()
+    # side by side is no overlap, and y may be x
+    at = dict(x=0, y=32, weight=64, bias=72, mean=80, rstd=84)
+    assert forward() == 0 and forward(y=0) == 0
+    at = dict(x=0, dy=32, weight=64, mean=72, rstd=76, dx=80, dweight=112, dbias=120)
+    assert backward() == 0
+    dev.wait()
+
+
 def test_refusals_without_a_device():
     f, b = ag.lib().ag_layer_norm_forward, ag.lib().ag_layer_norm_backward
     assert f(None, 0, None, None, None, 4, 8, EPS, None, None, None) == ag._capi.AG_ERR_INVALID
