@@ -77,55 +77,76 @@ static int launch(ag_device *dev, const CUtensorMap &map, __half *planes, double
     return AG_OK;
 }
 
-template <class T>
-int run(ag_device *dev, const std::vector<Matrix> &matrices, const Rule &rule, int steps) {
-    int taken = 0;
-    for (size_t first = 0; first < matrices.size(); first += taken) {
-        Group g = {};
+// One launch: its matrices, and what it takes of the workspace.
+struct Launch {
+    Group g;
+    int64_t space;       // rows of planes
+    int parts, blocks;   // CTAs of the passes before the steps
+    bool narrow;
+};
+
+// The launches that a list takes.
+static int make_launches(const std::vector<Matrix> &matrices, const Rule &rule, int steps, bool bf16, int sm_count,
+                         std::vector<Launch> &launches) {
+    for (size_t first = 0; first < matrices.size(); first += launches.back().g.n) {
+        launches.push_back({});
+        Launch &l = launches.back();
+        Group &g = l.g;
         g.steps = steps;
         g.rule = rule;
-        int64_t space = 0;
-        int parts = 0, blocks = 0;
         int64_t values = 0, tiles = 0;
         for (; g.n < kGroup && first + g.n < matrices.size(); ++g.n) {
             Matrix &m = g.m[g.n];
             m = matrices[first + g.n];
             const int64_t n = m.n(), wide = m.wide();
-            m.squares = squares_from(m, steps, sizeof(T) == 2);
-            if (g.n > 0 && space + m.space(steps) > kMostRows) break;
-            m.row = (int)std::min<int64_t>(space, INT32_MAX);
-            space += m.space(steps);
+            m.squares = squares_from(m, steps, bf16);
+            if (g.n > 0 && l.space + m.space(steps) > kMostRows) break;
+            m.row = (int)std::min<int64_t>(l.space, INT32_MAX);
+            l.space += m.space(steps);
             g.phases = std::max(g.phases, m.phases(steps));
-            m.part0 = parts;
+            m.part0 = l.parts;
             m.parts = (int)std::min<int64_t>(ceil_div(n * wide, 8192), kMostParts);
-            parts += m.parts;
-            blocks += m.x(0).plane / 64;
+            l.parts += m.parts;
+            l.blocks += m.x(0).plane / 64;
             values += n * wide;
             tiles += ceil_div(n, 128) * ceil_div(wide, 128);
         }
-        taken = g.n;
-        AG_REQUIRE(space < (1ll << 31), AG_ERR_LIMIT, "newton_schulz: the matrices' workspace is too large");
+        AG_REQUIRE(l.space < (1ll << 31), AG_ERR_LIMIT, "newton_schulz: the matrices' workspace is too large");
         g.inside = values <= kInside;
         // Tiles of 64 columns where wide ones would leave SMs idle: us, wide and narrow, f32 1024 x 1024 329 and 242, 512 x 512 230
         // and 165, 1536 x 1024 331 and 313; beyond a tile an SM wide ones win (two 1024 x 1024 and 700 x 700 405 and 451).
-        const bool narrow = tiles <= dev->sm_count;
-        const size_t heads = (size_t)kGroup * kMostParts * sizeof(double), sums = (size_t)dev->sm_count * 128 * 128 * sizeof(float);
-        void *ws;
-        AG_TRY(engine_scratch(dev, heads + sums + (size_t)space * 128, &ws));
-        double *norms = (double *)ws;
-        float4 *slices = (float4 *)((char *)ws + heads);
-        __half *planes = (__half *)((char *)ws + heads + sums);
-        CUtensorMap map;
-        const uint64_t dims[2] = {64, (uint64_t)space}, strides[1] = {64};
-        const uint32_t box[2] = {64, 64};
-        AG_TRY(make_tmap_bf16(&map, planes, 2, dims, strides, box));   // f16 has the same size
+        l.narrow = tiles <= sm_count;
+    }
+    return AG_OK;
+}
+
+// Nothing is launched before the whole list has its workspace: a call that fails has changed nothing.
+template <class T>
+int run(ag_device *dev, const std::vector<Matrix> &matrices, const Rule &rule, int steps) {
+    std::vector<Launch> launches;
+    AG_TRY(make_launches(matrices, rule, steps, sizeof(T) == 2, dev->sm_count, launches));
+    if (launches.empty()) return AG_OK;
+    int64_t space = 0;
+    for (const Launch &l : launches) space = std::max(space, l.space);
+    const size_t heads = (size_t)kGroup * kMostParts * sizeof(double), sums = (size_t)dev->sm_count * 128 * 128 * sizeof(float);
+    void *ws;
+    AG_TRY(engine_scratch(dev, heads + sums + (size_t)space * 128, &ws));
+    double *norms = (double *)ws;
+    float4 *slices = (float4 *)((char *)ws + heads);
+    __half *planes = (__half *)((char *)ws + heads + sums);
+    CUtensorMap map;
+    const uint64_t dims[2] = {64, (uint64_t)space}, strides[1] = {64};
+    const uint32_t box[2] = {64, 64};
+    AG_TRY(make_tmap_bf16(&map, planes, 2, dims, strides, box));   // f16 has the same size
+    for (const Launch &l : launches) {
+        const Group &g = l.g;
         if (!g.inside) {
-            momentum_kernel<T><<<parts, 256, 0, dev->stream>>>(g, norms);
+            momentum_kernel<T><<<l.parts, 256, 0, dev->stream>>>(g, norms);
             AG_CHECK_LAUNCH();
-            split_kernel<T><<<blocks, 256, 0, dev->stream>>>(g, norms, planes);
+            split_kernel<T><<<l.blocks, 256, 0, dev->stream>>>(g, norms, planes);
             AG_CHECK_LAUNCH();
         }
-        AG_TRY((narrow ? launch<T, 64>(dev, map, planes, norms, slices, g) : launch<T, 128>(dev, map, planes, norms, slices, g)));
+        AG_TRY((l.narrow ? launch<T, 64>(dev, map, planes, norms, slices, g) : launch<T, 128>(dev, map, planes, norms, slices, g)));
     }
     return AG_OK;
 }

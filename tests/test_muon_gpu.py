@@ -117,6 +117,31 @@ def test_a_list_larger_than_one_workspace(dev):
 
 
 @gpu
+def test_a_list_without_memory_for_its_last_matrix_changes_nothing(dev):
+    """33 matrices go in two launches, of which the second's workspace of 3 GB is not to be had: the first one's matrices keep
+    their weights and momenta too."""
+    dev.set_guards(False)
+    sizes = [(3, 5)] * 32 + [(8192, 16384)]
+    own = ag.Device(0)   # a device object whose workspace has not grown
+    torch.cuda.set_stream(own.stream)
+    w, g = [[torch.ones(s, device=own.torch_device, dtype=BF16) for s in sizes] for _ in range(2)]
+    v = [torch.zeros(s, device=own.torch_device) for s in sizes]
+    own.wait()
+    hog = []
+    try:
+        hog.append(torch.empty(torch.cuda.mem_get_info()[0] - (2 << 30), dtype=torch.uint8, device=own.torch_device))
+        with pytest.raises(ag.AgError) as err:
+            own.muon_update(w, g, v, 0.1)
+    finally:
+        hog.clear()
+        torch.cuda.empty_cache()
+        torch.cuda.set_stream(dev.stream)
+    own.wait()
+    assert err.value.status == ag._capi.AG_ERR_OOM
+    assert all((t == 1).all() for t in w) and not any(t.any() for t in v)
+
+
+@gpu
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 @pytest.mark.parametrize("rows,cols", [(40, 60), (300, 200), (200, 1500)])
 @pytest.mark.parametrize("steps", [1, 2, 3, 7])
