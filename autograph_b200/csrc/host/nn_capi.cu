@@ -10,6 +10,7 @@
 #include "../common.cuh"
 #include "../conv_chain.cuh"
 #include "../lenet_train.cuh"
+#include "../muon.cuh"
 #include "nn.hpp"
 #include "conv_stages.hpp"
 
@@ -965,23 +966,27 @@ float forward_backward(ag_model *m, const Tensor &x, const Tensor &t, float *los
 // Muon over all matrices in one call, SGD with momentum over the vectors.  A step of every matrix moves its outputs by about
 // as much whatever its shape: the factor sqrt(max(1, outputs / inputs)) with Dense weights [inputs, outputs] and filter banks
 // [outputs, inputs * filter].
-void muon_update(ag_model *m, float lr) {
+std::vector<ag_muon_matrix> muon_matrices(ag_model *m) {
     std::vector<ag_muon_matrix> list;
     for (size_t i = 0; i < m->params.size(); ++i) {
         Parameter *p = m->params[i];
-        const int64_t len = p->value.len();
-        if (p->value.ndim() < 2) {
-            check(ag_sgd_update_momentum(m->dev, m->dtype, p->value.data(), p->grad.data(), p->velocity.data(), len,
-                                         lr * m->muon.vector_scale, m->muon.momentum));
-            continue;
-        }
-        const int64_t rows = p->value.dim(0), cols = len / rows;
+        if (p->value.ndim() < 2) continue;
+        const int64_t rows = p->value.dim(0), cols = p->value.len() / rows;
         const double outs = (double)(p->value.ndim() == 2 ? cols : rows), ins = (double)(p->value.ndim() == 2 ? rows : cols);
         list.push_back({p->value.data(), p->grad.data(), (float *)m->muon.velocity.data() + m->offsets[i], rows, cols,
                         (float)std::sqrt(std::max(1.0, outs / ins))});
     }
+    return list;
+}
+void muon_update(ag_model *m, float lr) {
+    // the matrices first: only their update can be refused, and then nothing has moved
+    const std::vector<ag_muon_matrix> list = muon_matrices(m);
     check(ag_muon_update(m->dev, m->dtype, (int32_t)list.size(), list.data(), lr, m->muon.momentum, m->muon.nesterov,
                          m->muon.weight_decay, m->muon.steps));
+    for (Parameter *p : m->params)
+        if (p->value.ndim() < 2)
+            check(ag_sgd_update_momentum(m->dev, m->dtype, p->value.data(), p->grad.data(), p->velocity.data(), p->value.len(),
+                                         lr * m->muon.vector_scale, m->muon.momentum));
 }
 
 // ≙ model.update(lr, &sgd) (layer.rs:656-658 -> SGD::update, optimizer.rs:389-428), over the
@@ -1360,11 +1365,9 @@ int ag_model_set_muon(ag_model *model, float momentum, int nesterov, float weigh
     AG_REQUIRE(weight_decay == weight_decay && vector_scale == vector_scale, AG_ERR_INVALID, "muon: a scalar is no number");
     AG_ENTER(model->dev);
     AG_HOST_GUARD({
-        for (Parameter *p : model->params)
-            if (p->value.ndim() >= 2 && std::min(p->value.dim(0), p->value.len() / p->value.dim(0)) > 16384)
-                throw Error(AG_ERR_LIMIT, "muon: a parameter's shorter side is beyond 16384");
         if (!model->muon.velocity.defined())
             model->muon.velocity = Tensor::uninit(model->pool, {model->bucket_len}, AG_F32);
+        check(::ag::muon_prepare(model->dev, model->dtype, muon_matrices(model), steps));
         check(ag_fill_zero(model->dev, model->muon.velocity.data(), model->muon.velocity.nbytes()));
         check(ag_fill_zero(model->dev, model->velocity.data(), model->velocity.nbytes()));
         model->muon.on = true;

@@ -8,6 +8,7 @@
 #include <algorithm>
 #include <vector>
 
+#include "muon.cuh"
 #include "muon_product.cuh"
 
 namespace ag {
@@ -120,33 +121,47 @@ static int make_launches(const std::vector<Matrix> &matrices, const Rule &rule, 
     return AG_OK;
 }
 
+// The workspace of all launches of a call, one after the other.
+struct Space {
+    double *norms;
+    float4 *slices;
+    __half *planes;
+    int64_t rows;   // of the planes
+};
+static int take_space(ag_device *dev, const std::vector<Launch> &launches, Space &s) {
+    s.rows = 0;
+    for (const Launch &l : launches) s.rows = std::max(s.rows, l.space);
+    const size_t heads = (size_t)kGroup * kMostParts * sizeof(double), sums = (size_t)dev->sm_count * 128 * 128 * sizeof(float);
+    void *ws;
+    AG_TRY(engine_scratch(dev, heads + sums + (size_t)s.rows * 128, &ws));
+    s.norms = (double *)ws;
+    s.slices = (float4 *)((char *)ws + heads);
+    s.planes = (__half *)((char *)ws + heads + sums);
+    return AG_OK;
+}
+
 // Nothing is launched before the whole list has its workspace: a call that fails has changed nothing.
 template <class T>
 int run(ag_device *dev, const std::vector<Matrix> &matrices, const Rule &rule, int steps) {
     std::vector<Launch> launches;
     AG_TRY(make_launches(matrices, rule, steps, sizeof(T) == 2, dev->sm_count, launches));
     if (launches.empty()) return AG_OK;
-    int64_t space = 0;
-    for (const Launch &l : launches) space = std::max(space, l.space);
-    const size_t heads = (size_t)kGroup * kMostParts * sizeof(double), sums = (size_t)dev->sm_count * 128 * 128 * sizeof(float);
-    void *ws;
-    AG_TRY(engine_scratch(dev, heads + sums + (size_t)space * 128, &ws));
-    double *norms = (double *)ws;
-    float4 *slices = (float4 *)((char *)ws + heads);
-    __half *planes = (__half *)((char *)ws + heads + sums);
+    Space s;
+    AG_TRY(take_space(dev, launches, s));
     CUtensorMap map;
-    const uint64_t dims[2] = {64, (uint64_t)space}, strides[1] = {64};
+    const uint64_t dims[2] = {64, (uint64_t)s.rows}, strides[1] = {64};
     const uint32_t box[2] = {64, 64};
-    AG_TRY(make_tmap_bf16(&map, planes, 2, dims, strides, box));   // f16 has the same size
+    AG_TRY(make_tmap_bf16(&map, s.planes, 2, dims, strides, box));   // f16 has the same size
     for (const Launch &l : launches) {
         const Group &g = l.g;
         if (!g.inside) {
-            momentum_kernel<T><<<l.parts, 256, 0, dev->stream>>>(g, norms);
+            momentum_kernel<T><<<l.parts, 256, 0, dev->stream>>>(g, s.norms);
             AG_CHECK_LAUNCH();
-            split_kernel<T><<<l.blocks, 256, 0, dev->stream>>>(g, norms, planes);
+            split_kernel<T><<<l.blocks, 256, 0, dev->stream>>>(g, s.norms, s.planes);
             AG_CHECK_LAUNCH();
         }
-        AG_TRY((l.narrow ? launch<T, 64>(dev, map, planes, norms, slices, g) : launch<T, 128>(dev, map, planes, norms, slices, g)));
+        AG_TRY((l.narrow ? launch<T, 64>(dev, map, s.planes, s.norms, s.slices, g)
+                         : launch<T, 128>(dev, map, s.planes, s.norms, s.slices, g)));
     }
     return AG_OK;
 }
@@ -190,6 +205,23 @@ static int check_overlap(std::vector<Range> &ranges) {
 }
 
 }  // namespace muon
+
+int muon_prepare(ag_device *dev, ag_dtype dtype, const std::vector<ag_muon_matrix> &matrices, int steps) {
+    AG_REQUIRE(matrices.size() <= (size_t)muon::kMostMatrices, AG_ERR_LIMIT, "muon: %zu matrices, at most %d", matrices.size(),
+               muon::kMostMatrices);
+    if (matrices.empty()) return AG_OK;
+    AG_TRY(muon::check_call(dtype, (int32_t)matrices.size(), matrices.data(), steps));
+    std::vector<muon::Matrix> list;
+    for (const ag_muon_matrix &m : matrices) {
+        AG_TRY(muon::check_size(m.rows, m.cols));
+        list.push_back({m.g, m.w, m.v, m.rows, m.cols, m.scale, 0, 0, 0, 0});
+    }
+    std::vector<muon::Launch> launches;
+    AG_TRY(muon::make_launches(list, {}, steps, dtype == AG_BF16, dev->sm_count, launches));
+    muon::Space space;
+    return muon::take_space(dev, launches, space);
+}
+
 }  // namespace ag
 
 using namespace ag;

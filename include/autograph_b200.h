@@ -544,7 +544,8 @@ AG_API int ag_model_get_velocity(ag_model *model, int32_t index, void *host);
 AG_API int ag_model_set_velocity(ag_model *model, int32_t index, const void *host);
 /* Muon (ag_muon_update) for every parameter of two dimensions or more, all in one call, with the
  * factor sqrt(max(1, outputs / inputs)) on each; vectors (biases, LayerNorm) take SGD with the same
- * momentum and lr * vector_scale.  Clears the momenta.  ag_model_set_sgd goes back.  A step then
+ * momentum and lr * vector_scale.  Clears the momenta.  Refuses a model with parameters beyond
+ * ag_muon_update's limits, and takes the workspace of the updates.  ag_model_set_sgd goes back.  A step then
  * takes the same calls as with SGD, except ag_model_allreduce_update (AG_ERR_UNSUPPORTED: all-reduce
  * the bucket and call ag_model_apply_update). */
 AG_API int ag_model_set_muon(ag_model *model, float momentum, int nesterov, float weight_decay,

@@ -233,6 +233,40 @@ def test_refusals(dev):
     assert lib.ag_model_set_muon(None, 0.9, 1, 0.0, 5, 1.0) == inv
 
 
+def test_parameters_beyond_the_limits_are_refused_at_set_muon(dev):
+    """At once, not by every step after its vectors have moved: a longer side above 2^20."""
+    m = ag.Model(dev, [("flatten",), ("dense", 1, (1 << 20) + 1, True)], F32, seed=1)
+    m.set_sgd(0.5)
+    m.set_velocities([np.ones(n, np.float32) for n in m.parameter_lens])
+    with pytest.raises(ag.AgError) as err:
+        m.set_muon()
+    assert err.value.status == ag._capi.AG_ERR_LIMIT
+    # the model keeps its optimizer and that one's state
+    assert m.muon is None and m.momentum == 0.5
+    assert all((m.get_velocity(i) == 1).all() for i in range(2))
+
+
+def test_set_muon_takes_the_updates_workspace(dev):
+    """No step fails for want of memory after some of it: where there is none for the workspace, set_muon says so."""
+    dev.set_guards(False)
+    own = ag.Device(0)
+    torch.cuda.set_stream(own.stream)
+    hog = []
+    try:
+        m = ag.Model(own, [("flatten",), ("dense", 8192, 8192, False)], BF16, seed=1)   # planes of 1.07 GB
+        own.wait()
+        # room for the momenta of 268 MB alone
+        hog.append(torch.empty(torch.cuda.mem_get_info()[0] - (1 << 30), dtype=torch.uint8, device=own.torch_device))
+        with pytest.raises(ag.AgError) as err:
+            m.set_muon()
+        assert err.value.status == ag._capi.AG_ERR_OOM
+    finally:
+        hog.clear()
+        torch.cuda.empty_cache()
+        torch.cuda.set_stream(dev.stream)
+    m.set_muon()
+
+
 def test_two_models_on_two_devices_of_one_gpu(dev):
     """Two threads, each with a device of its own: kernels that need the whole GPU do not wait for each other's halves."""
     import threading
