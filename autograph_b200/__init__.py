@@ -1064,17 +1064,22 @@ class _PyModel:
                                           optimizer="Muon" if muon else "SGD"))
 
     def load_serde_json(self, text: str):
-        """Loads the parameters of a stack written by to_serde_json or by the reference."""
+        """Loads the parameters of a stack written by to_serde_json or by the reference, and their state where it is that
+        of the model's optimizer.  After the state of another one (SGD's under Muon, or Muon's under SGD with momentum) the
+        momenta start at zero."""
         from . import serde_format as sf
-        params, states = sf.model_from_value(sf.loads(text), with_state=True)
+        value = sf.loads(text)
+        params, states = sf.model_from_value(value, with_state=True)
         if [p.size for p in params] != list(self.parameter_lens):
             raise AgError(_capi.AG_ERR_SHAPE, "checkpoint does not match the model's parameters")
         self.set_parameters(params)
-        if all(v is not None for v in states):   # a momentum run continues where it stopped
-            if getattr(self, "muon", None) is not None:
-                self.set_momenta(states)
-            elif getattr(self, "momentum", None):
-                self.set_velocities(states)
+        muon = getattr(self, "muon", None) is not None
+        if not muon and not getattr(self, "momentum", None):
+            return
+        if sf.optimizers_of(value) - {"Muon" if muon else "SGD"}:
+            self.set_momenta([np.zeros(n, np.float32) for n in self.parameter_lens])
+        elif all(v is not None for v in states):   # a momentum run continues where it stopped
+            (self.set_momenta if muon else self.set_velocities)(states)
 
     def forward_device(self, x_dev, out_dev=None):
         bs, c, h, w = x_dev.shape

@@ -179,10 +179,17 @@ def model_to_value(spec, params, field_names, bf16: bool = False, velocities=Non
     return out
 
 
+def optimizers_of(value: dict) -> set:
+    """The names of the optimizers whose state a stack's parameters carry."""
+    layers = [layer for layer in value.values() if isinstance(layer, dict)]
+    states = [(layer.get(key) or {}).get("optim_state") for layer in layers for key in ("weight", "bias")]
+    return {state.get("name") for state in states if state}
+
+
 def model_from_value(value: dict, with_state: bool = False):
     """The parameter arrays (float32, flattened, in field order: weight then bias) of a stack
-    written by model_to_value or by the reference.  with_state: also the list of SGD velocities
-    (None where a parameter carries no state)."""
+    written by model_to_value or by the reference.  with_state: also the list of velocities
+    (None where a parameter carries no state), whichever optimizer wrote them (optimizers_of)."""
     params, states = [], []
     for layer in value.values():
         if not isinstance(layer, dict):

@@ -214,6 +214,29 @@ def test_muon_continues_from_a_checkpoint(dev, dtype):
         assert (a.get_parameter(i) == b.get_parameter(i)).all() and (a.get_momentum(i) == b.get_momentum(i)).all()
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("to_muon", [True, False], ids=["sgd_to_muon", "muon_to_sgd"])
+def test_another_optimizers_checkpoint(dev, dtype, to_muon):
+    """The parameters load; the state is not the model's own, so that its momenta start at zero, as set_muon and set_sgd leave
+    them."""
+    dev.set_guards(False)
+    a, b, c = (_model(dev, dtype, seed=s) for s in (3, 8, 9))
+    set_other, set_own = (lambda m: m.set_sgd(0.9)), (lambda m: m.set_muon(momentum=0.9))
+    if not to_muon:
+        set_other, set_own = set_own, set_other
+    set_other(a), set_own(b), set_own(c)
+    for m in (a, b):
+        m.train_step(*_batch(16, dtype), 0.02)
+    b.load_serde_json(a.to_serde_json(NAMES))
+    c.set_parameters([a.get_parameter(i) for i in range(len(SHAPES))])
+    for i in range(len(SHAPES)):
+        assert (b.get_parameter(i) == a.get_parameter(i)).all() and not b.get_momentum(i).any()
+    for m in (b, c):
+        m.train_step(*_batch(16, dtype, seed=1), 0.02)
+    for i in range(len(SHAPES)):
+        assert (b.get_parameter(i) == c.get_parameter(i)).all()
+
+
 def test_refusals(dev):
     m = _model(dev, F32)
     inv, uns = ag._capi.AG_ERR_INVALID, ag._capi.AG_ERR_UNSUPPORTED

@@ -56,6 +56,18 @@ def test_model_round_trip_f32_and_bf16():
     assert all(np.array_equal(a.ravel(), b) for a, b in zip(pb, back))
 
 
+@pytest.mark.parametrize("name", ["SGD", "Muon"])
+def test_whose_state_a_checkpoint_holds(name):
+    spec = [("dense", 3, 4, True), ("relu",), ("layer_norm", 4, False)]
+    params = [np.ones(n, np.float32) for n in (12, 4, 4)]
+    plain = sf.model_to_value(spec, params, ["a", "b", "c"])
+    assert sf.optimizers_of(plain) == set()
+    v = sf.loads(sf.dumps(sf.model_to_value(spec, params, ["a", "b", "c"], velocities=params, optimizer=name)))
+    assert sf.optimizers_of(v) == {name}
+    v["c"]["weight"]["optim_state"]["name"] = "Other"
+    assert sf.optimizers_of(v) == {name, "Other"}
+
+
 def test_optimizer_state_layout_and_round_trip():
     """Parameter { value, optim_state } with SGD's velocity (autograd.rs:647-656,
     optimizer.rs:102-131, 166-172, 366-383): State { name, key_values: [("velocity",
