@@ -32,6 +32,8 @@ import json
 
 import numpy as np
 
+NORM_EPS = 1e-5   # of every LayerNorm layer
+
 _NAMES = {"uint8": "U8", "int8": "I8", "uint16": "U16", "int16": "I16", "uint32": "U32",
           "int32": "I32", "uint64": "U64", "int64": "I64", "float16": "F16", "float32": "F32",
           "float64": "F64"}
@@ -168,7 +170,7 @@ def model_to_value(spec, params, field_names, bf16: bool = False, velocities=Non
         elif kind == "layer_norm":   # not a layer of the reference: the layout of its other layers
             w = np.asarray(next(it), np.float32).reshape(layer[1])
             b = np.asarray(next(it), np.float32).reshape(layer[1]) if layer[2] else None
-            out[name] = {"weight": param(w), "bias": param(b) if layer[2] else None, "eps": 1e-5}
+            out[name] = {"weight": param(w), "bias": param(b) if layer[2] else None, "eps": NORM_EPS}
         elif kind == "pool":
             out[name] = {"filter": [int(layer[1][0]), int(layer[1][1])],
                          "stride": [int(layer[1][0]), int(layer[1][1])]}
@@ -194,6 +196,8 @@ def model_from_value(value: dict, with_state: bool = False):
     for layer in value.values():
         if not isinstance(layer, dict):
             continue
+        if np.float32(layer.get("eps", NORM_EPS)) != np.float32(NORM_EPS):
+            raise ValueError(f"a layer norm with eps {layer['eps']}: the layers here have {NORM_EPS}")
         for key in ("weight", "bias"):
             p = layer.get(key)
             if p is None:

@@ -56,6 +56,19 @@ def test_model_round_trip_f32_and_bf16():
     assert all(np.array_equal(a.ravel(), b) for a, b in zip(pb, back))
 
 
+def test_a_norm_with_another_eps_is_refused():
+    """Its outputs would not be those of the layer that was saved."""
+    v = sf.model_to_value([("layer_norm", 4, True)], [np.ones(4, np.float32), np.zeros(4, np.float32)], ["n"])
+    assert v["n"]["eps"] == 1e-5
+    for eps in (1e-5, float(np.float32(1e-5))):   # as 64 and as 32 bits are printed
+        v["n"]["eps"] = eps
+        assert len(sf.model_from_value(sf.loads(sf.dumps(v)))) == 2
+    for eps in (1e-6, 1e-3, 0.0):
+        v["n"]["eps"] = eps
+        with pytest.raises(ValueError, match="eps"):
+            sf.model_from_value(v)
+
+
 @pytest.mark.parametrize("name", ["SGD", "Muon"])
 def test_whose_state_a_checkpoint_holds(name):
     spec = [("dense", 3, 4, True), ("relu",), ("layer_norm", 4, False)]
