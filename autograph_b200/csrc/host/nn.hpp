@@ -496,8 +496,9 @@ class LayerNorm : public Layer {
         const int64_t size = weight.value.len();
         int64_t cols = 1;
         size_t d = x.ndim();
-        while (d > 1 && cols < size) cols *= x.dim(--d);
-        if (cols != size)
+        // at least the last dimension, never the batch
+        while (d > 1 && (cols < size || d == x.ndim())) cols *= x.dim(--d);
+        if (cols != size || d == x.ndim())
             throw Error(AG_ERR_SHAPE, "LayerNorm: the input's trailing dimensions do not hold " + std::to_string(size) +
                                           " values");
         if (!x.is_standard_layout()) throw Error(AG_ERR_SHAPE, "LayerNorm needs standard layout");

@@ -103,6 +103,23 @@ def test_sizes_that_no_trailing_dimensions_have(dev):
         ag.Model(dev, [("layer_norm", 0, True), ("flatten",), ("dense", 144, 10, True)])
 
 
+def test_a_norm_of_one_value_a_row(dev):
+    """It takes inputs whose last dimension is one, and gives the bias; others have rows of more than one value."""
+    x, _ = _batch(2, F32)
+    with pytest.raises(ag.AgError) as err:
+        ag.Model(dev, [("layer_norm", 1, True), ("flatten",), ("dense", 144, 10, True)]).infer(x)
+    assert err.value.status == ag._capi.AG_ERR_SHAPE
+    with pytest.raises(ag.AgError) as err:
+        ag.Model(dev, [("flatten",), ("dense", 144, 10, True), ("layer_norm", 1, True)]).infer(x)
+    assert err.value.status == ag._capi.AG_ERR_SHAPE
+    m = ag.Model(dev, [("flatten",), ("dense", 144, 1, True), ("layer_norm", 1, True), ("dense", 1, 10, True)])
+    bias = np.float32(0.25)
+    m.set_parameters([m.get_parameter(0), m.get_parameter(1), np.ones(1, np.float32), np.full(1, bias), m.get_parameter(4),
+                      m.get_parameter(5)])
+    want = bias * m.get_parameter(4) + m.get_parameter(5)
+    assert np.abs(m.infer(x).numpy() - want).max() <= 4 * 2.0 ** -24 * (np.abs(m.get_parameter(4)).max() + 1)
+
+
 def _polar64(g, steps):
     x = g / g.norm() if g.norm() > 0 else g
     flip = g.shape[0] > g.shape[1]
