@@ -108,7 +108,8 @@ inline size_t sym_bytes(int world) { return 2 * (size_t)world * kCapWords * 8; }
 
 // One member GPU of a communicator, as this process sees it.
 struct ag_comm_member {
-    ag_device *dev = nullptr;      // the rank's device object (ordinal + stream); not owned
+    ag_device *dev = nullptr;      // the rank's device object (ordinal + stream)
+    ag::DeviceRef keep;
     ag::nccl_comm_t nccl = nullptr;
     void *sym = nullptr;           // this rank's symmetric block (owned when local)
     void *peer_sym[ag::kMaxRanks] = {};  // every rank's block as addressable from this rank
@@ -376,6 +377,7 @@ int ag_comm_create(ag_device *const *devs, int n, ag_comm **out) {
     }
     for (int i = 0; i < n; ++i) {
         c->members[(size_t)i].dev = devs[i];
+        c->members[(size_t)i].keep = ag::DeviceRef(devs[i]);
         c->members[(size_t)i].nccl = comms[(size_t)i];
     }
     // Symmetric blocks: every GPU maps every other GPU's block through peer access.
@@ -423,6 +425,7 @@ int ag_comm_create_rank(ag_device *dev, int world, int rank, const void *unique_
     c->members.resize(1);
     ag_comm_member &m = c->members[0];
     m.dev = dev;
+    m.keep = DeviceRef(dev);
     m.nccl = nc;
     *out = c;
     // Symmetric block: exchange CUDA IPC handles with an all-gather, then map the peers'.

@@ -9,6 +9,7 @@
 #include <cstdint>
 #include <cstdio>
 #include <mutex>
+#include <utility>
 #include <vector>
 
 #include "../../include/autograph_b200.h"
@@ -65,6 +66,7 @@ constexpr int kTileCounters = 1024;
 // split-k GEMM use for partial sums, a device status word that bounded device
 // waits report into, and a pinned host word for scalar read-backs.
 struct ag_device {
+    std::atomic<int> refs{1};       // its creator, and the models and communicators on it (DeviceRef)
     int ordinal = 0;
     cudaStream_t stream = nullptr;
     bool owns_stream = false;
@@ -176,6 +178,27 @@ __device__ __forceinline__ void signal_done(const Done &d) {
     }
     *reinterpret_cast<volatile uint32_t *>(d.flag) = d.seq;
 }
+
+// Frees the device object with the last reference to it.
+void device_release(ag_device *dev);
+
+// Keeps a device object for an owner that is destroyed after it: a garbage collector takes objects in any order.
+class DeviceRef {
+   public:
+    DeviceRef() = default;
+    explicit DeviceRef(ag_device *dev) : dev_(dev) { dev_->refs.fetch_add(1, std::memory_order_relaxed); }
+    DeviceRef(DeviceRef &&o) noexcept : dev_(o.dev_) { o.dev_ = nullptr; }
+    DeviceRef &operator=(DeviceRef &&o) noexcept {
+        std::swap(dev_, o.dev_);
+        return *this;
+    }
+    ~DeviceRef() {
+        if (dev_) device_release(dev_);
+    }
+
+   private:
+    ag_device *dev_ = nullptr;
+};
 
 // Makes `dev` current on the calling thread and locks it for the call.
 class DeviceGuard {

@@ -71,6 +71,7 @@ struct TrainEntry {
 };
 
 struct ag_model {
+    ::ag::DeviceRef keep;   // first, so that it is the last to go
     ag_device *dev;
     ag_dtype dtype;
     Pool pool;  // declared before every tensor so that it is destroyed last
@@ -122,7 +123,7 @@ struct ag_model {
     uint64_t muon_settings = 0;   // how often Muon was set
     uint64_t muon_rule() const { return muon.on ? muon_settings : 0; }
     float grad_scale = 1.f;
-    ag_model(ag_device *d, ag_dtype t) : dev(d), dtype(t), pool(d) {
+    ag_model(ag_device *d, ag_dtype t) : keep(d), dev(d), dtype(t), pool(d) {
         const char *e = getenv("AG_GRAPH");
         graphs_enabled = !(e && e[0] == '0');
         const char *z = getenv("AG_ZERO_COPY");

@@ -90,6 +90,24 @@ int engine_scratch(ag_device *dev, size_t bytes, void **out) {
     return AG_OK;
 }
 
+void device_release(ag_device *dev) {
+    if (dev->refs.fetch_sub(1, std::memory_order_acq_rel) != 1) return;
+    cudaSetDevice(dev->ordinal);
+    if (dev->stream) cudaStreamSynchronize(dev->stream);
+    if (dev->workspace) cudaFree(dev->workspace);
+    if (dev->staging) cudaFree(dev->staging);
+    if (dev->engine) cudaFree(dev->engine);
+    for (void *p : dev->retired) cudaFree(p);
+    if (dev->status_dev) cudaFree(dev->status_dev);
+    if (dev->tile_counters) cudaFree(dev->tile_counters);
+    if (dev->scalar_dev) cudaFree(dev->scalar_dev);
+    if (dev->status_host) cudaFreeHost(dev->status_host);
+    if (dev->scalar_host) cudaFreeHost(dev->scalar_host);
+    if (dev->done_host) cudaFreeHost((void *)dev->done_host);
+    if (dev->owns_stream && dev->stream) cudaStreamDestroy(dev->stream);
+    delete dev;
+}
+
 static int device_init(int ordinal, cudaStream_t stream, bool owns, ag_device **out) {
     AG_REQUIRE(out != nullptr, AG_ERR_INVALID, "out is null");
     int count = 0;
@@ -194,18 +212,7 @@ int ag_device_destroy(ag_device *dev) {
     if (!dev) return AG_OK;
     cudaSetDevice(dev->ordinal);
     if (dev->stream) cudaStreamSynchronize(dev->stream);
-    if (dev->workspace) cudaFree(dev->workspace);
-    if (dev->staging) cudaFree(dev->staging);
-    if (dev->engine) cudaFree(dev->engine);
-    for (void *p : dev->retired) cudaFree(p);
-    if (dev->status_dev) cudaFree(dev->status_dev);
-    if (dev->tile_counters) cudaFree(dev->tile_counters);
-    if (dev->scalar_dev) cudaFree(dev->scalar_dev);
-    if (dev->status_host) cudaFreeHost(dev->status_host);
-    if (dev->scalar_host) cudaFreeHost(dev->scalar_host);
-    if (dev->done_host) cudaFreeHost((void *)dev->done_host);
-    if (dev->owns_stream && dev->stream) cudaStreamDestroy(dev->stream);
-    delete dev;
+    device_release(dev);
     return AG_OK;
 }
 

@@ -82,6 +82,8 @@ AG_API int ag_device_count(int *count);
 AG_API int ag_device_create(int ordinal, ag_device **out);
 /* Same, but work is submitted to a stream the caller owns (cudaStream_t). */
 AG_API int ag_device_create_on_stream(int ordinal, void *cuda_stream, ag_device **out);
+/* The handle is not used again; the object itself lives on until the models and communicators on it
+ * are destroyed, in whichever order that happens (and with it needs the stream that it was created on). */
 AG_API int ag_device_destroy(ag_device *dev);
 /* ≙ device.wait() (src/tensor/linalg.rs:549). Also reports a device-side timeout flag. */
 AG_API int ag_device_wait(ag_device *dev);

@@ -63,6 +63,25 @@ def abi():
     a.close()
 
 
+def test_a_model_outlives_its_device_handle(abi):
+    """A garbage collector takes a device object and the models on it in any order: the model works on, and the last of them
+    to go frees the device's buffers."""
+    lib = abi.lib
+    h, m = ctypes.c_void_p(), ctypes.c_void_p()
+    _capi.check(lib.ag_device_create(0, ctypes.byref(h)))
+    _capi.check(lib.ag_model_create_lenet5(h, _capi.AG_F32, 1, ctypes.byref(m)))
+    x = np.random.default_rng(0).uniform(0, 1, (4, 1, 28, 28)).astype(np.float32)
+    before, after = np.empty((4, 10), np.float32), np.empty((4, 10), np.float32)
+    _capi.check(lib.ag_model_infer(m, x.ctypes.data, 4, 1, 28, 28, before.ctypes.data))
+    _capi.check(lib.ag_device_destroy(h))
+    _capi.check(lib.ag_model_infer(m, x.ctypes.data, 4, 1, 28, 28, after.ctypes.data))
+    assert np.array_equal(before, after) and np.isfinite(before).all()
+    _capi.check(lib.ag_model_destroy(m))
+    p = abi.alloc(64)   # nothing is left behind for the thread's next calls
+    _capi.check(lib.ag_fill_zero(abi.dev, p, 64))
+    _capi.check(lib.ag_device_wait(abi.dev))
+
+
 def test_device_object(abi):
     lib = abi.lib
     n = ctypes.c_int()
