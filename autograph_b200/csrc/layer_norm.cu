@@ -14,8 +14,8 @@
 // A backward group takes every `groups`-th row and adds dy * hat and dy of its columns in registers as it goes; the CTAs'
 // sums are added in the order of the CTAs, by the CTA that finishes last or, where there is more to add, by a second
 // kernel.  Longer rows take two kernels that read them again.
-// Of the measured copy bandwidth, 65536 x 1024: f32 forward 0.97 (85 us), backward 0.91 (136), bf16 0.86 (48) and 0.72 (86: a
-// quarter of the warps, whose 128 registers hold row and sums); 256 x 25088 f32 forward 0.65 (12 us in L2, one row an SM at a time).
+// Of the measured copy bandwidth, 65536 x 1024: f32 forward 0.95 (87 us), backward 0.90 (137), bf16 0.79 (52) and 0.70 (88: a
+// quarter of the warps, whose 128 registers hold row and sums); 256 x 25088 f32 forward 0.43 (18 us: one row an SM at a time).
 //
 // Products that feed a sum are written as __fmul_rn or fmaf: left to the compiler, it fuses them one way in the loop for calls
 // that ask for the statistics, or for one gradient, and another way in the next, and the same values would give other bits.
@@ -87,7 +87,7 @@ constexpr int threads_of() { return G == 32 ? 256 : G; }
 // From the sums of the differences from a first mean, and of their squares: the mean, put right by what the differences leave, and
 // 1 / sqrt(variance + eps).  The first mean is off by the roundings of a sum of n values, 1e-5 of it for 25088 equal ones; what
 // these differences leave is off by the same share of them, so that of equal values the mean is that value and y is the bias.
-// us with and without: bf16 65536 x 1024 54.9 and 51.8, f32 256 x 25088 18.1 and 17.1.
+// us with and without: bf16 65536 x 1024 52 to 55 and 51.8, 2048 x 25088 55 and 51, f32 256 x 25088 18.1 and 17.1.
 __device__ __forceinline__ float finish_statistics(const float (&e)[2], float n, float eps, float &mean) {
     const float left = __fdiv_rn(e[0], n), var = fmaf(-left, left, __fdiv_rn(e[1], n));
     mean += left;
@@ -493,7 +493,7 @@ struct Backward {
 };
 
 // The kernel whose registers hold a row.  With vectors as few threads as can hold it: a row of a warp needs no barrier, and what a
-// row of a CTA waits at its barriers other rows of the SM fill.  us, with 256 threads or more from 1024 columns on, and so: bf16
+// row of a CTA waits at its barriers other rows of the SM fill.  us (taken before finish_statistics put the mean right), with 256 threads or more from 1024 columns on, and so: bf16
 // forward 32768 x 2048 95.6 and 50.1, 16384 x 4096 67.2 and 50.6, 8192 x 8192 73.2 and 53.8, backward 162 and 115.  Single values
 // would be many loads of few threads: f32 4093 x 2011 forward 17.8 with 256 threads, 24.1 with 128, backward 27.9 and 36.9.
 template <int VEC, class F>

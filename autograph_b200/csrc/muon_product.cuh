@@ -14,9 +14,9 @@
 // runs along the rows.
 //
 // What bounds it.  Small matrices: latency, 7 to 8 us a phase of fifteen (the barrier about 3, the first products 1.7, their
-// read-out and stores 1.5; LeNet5's five weights f32 127 us; a CTA a matrix without the barrier took 242).  Large ones: what a
-// tile of 128 x 128 reads of L2, 64 KB for 768 cycles of products of two planes, and the read-out where one plane is multiplied:
-// 4096 x 4096 bf16 2.85 ms of 1.50 at the measured bf16 rate, 1024 x 1024 f32 242 us of 39.  One launch a product, dependent
+// read-out and stores 1.5; LeNet5's five weights f32 120 us; a CTA a matrix without the barrier took 242).  Large ones: what a
+// tile of 128 x 128 reads of L2, 64 KB for 768 cycles of products: 4096 x 4096 bf16 4.3 ms of 2.5 at the measured bf16 rate,
+// 1024 x 1024 f32 227 us of 39.  One launch a product, dependent
 // or not, cost 10 us each where a phase costs 8.
 #pragma once
 

@@ -107,6 +107,20 @@ def test_both_directions(dev, rows, cols, dtype):
 
 @gpu
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("rows,cols", [(20000, 1), (30001, 2), (8192, 3), (12345, 5), (60000, 8), (65536, 16)])
+def test_many_short_rows(dev, rows, cols, dtype):
+    """The column sums come from every thread block there is room for."""
+    x, w, b, dy = _inputs(dev, rows, cols, dtype, seed=rows + cols)
+    y, mean, rstd = dev.layer_norm_keep(x, w, b, eps=EPS)
+    _check_forward(x, w, b, y, mean, rstd)
+    grads = dev.layer_norm_backward(x, dy, mean, rstd, w, has_bias=True)
+    _check_backward(x, w, mean, rstd, dy, *grads)
+    again = dev.layer_norm_backward(x, dy, mean, rstd, w, has_bias=True)
+    assert all(torch.equal(a, c) for a, c in zip(grads, again))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 @pytest.mark.parametrize("rows,cols", [(100, 84), (65, 1021), (3, 25088)])
 @pytest.mark.parametrize("has_w,has_b", [(False, False), (True, False), (False, True)])
 def test_without_weight_or_bias(dev, rows, cols, dtype, has_w, has_b):
