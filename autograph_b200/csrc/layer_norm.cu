@@ -493,9 +493,10 @@ struct Backward {
 };
 
 // The kernel whose registers hold a row.  With vectors as few threads as can hold it: a row of a warp needs no barrier, and what a
-// row of a CTA waits at its barriers other rows of the SM fill.  us (taken before finish_statistics put the mean right), with 256 threads or more from 1024 columns on, and so: bf16
+// row of a CTA waits at its barriers other rows of the SM fill.  us, with 256 threads or more from 1024 columns on, and so: bf16
 // forward 32768 x 2048 95.6 and 50.1, 16384 x 4096 67.2 and 50.6, 8192 x 8192 73.2 and 53.8, backward 162 and 115.  Single values
 // would be many loads of few threads: f32 4093 x 2011 forward 17.8 with 256 threads, 24.1 with 128, backward 27.9 and 36.9.
+// (Forward figures here and below are from before the sum of the differences, which adds up to a tenth to either side.)
 template <int VEC, class F>
 int forward_by_columns(const F &f) {
     const int64_t n = f.cols;
